@@ -30,6 +30,8 @@
  *       experts split by id (no counterpart in the reference)
  *   vqmoe_add_rms_norm      the decoder's residual add + RMSNorm
  *       (qwen3_5.py:120-130, 578-587)
+ *   vqmoe_quantize_fp8, vqmoe_grouped_linear  block-scaled e4m3 and ragged
+ *       grouped products (no counterpart in the reference)
  *
  * Numerics (matching the reference's rounding order, qwen3_5.py:35-40,
  * 108-112, 170-192): bf16 matmul outputs; fp32 softmax / top-k /
@@ -89,7 +91,7 @@ enum {
                                     IN/group]; codebook [K, dim] fp16 with dim
                                     2, 4 or 8, K <= 65536 (the wider formats
                                     the tiled fast path does not take) */
-    VQMOE_FMT_AFFINE = 3         /* affine-quantized experts, mlx-lm's
+    VQMOE_FMT_AFFINE = 3,        /* affine-quantized experts, mlx-lm's
                                     QuantizedSwitchLinear (switch_layers.py:
                                     24-86, mx.gather_qmm mode "affine"):
                                     weight [E, OUT, IN*bits/32] uint32, each row
@@ -98,6 +100,13 @@ enum {
                                     (j+1)*bits)); scales and biases [E, OUT,
                                     IN/group] bf16; W = bf16(fmaf(scale, q,
                                     bias)); activations stay bf16 */
+    VQMOE_FMT_FP8_BLOCK = 4      /* block-scaled e4m3 experts: weight [E, OUT,
+                                    IN] float8 e4m3fn, scales [E, ceil(OUT/128),
+                                    ceil(IN/128)] float32, one for each 128 x 128
+                                    block (weight_scale_inv of a block-quantized
+                                    checkpoint); group_size 128. Activations are
+                                    quantized to e4m3 with a float32 scale for
+                                    each row and 128 inputs (vqmoe_quantize_fp8) */
 };
 
 /* One switch linear: y[r] = x[r] @ W[expert(r)]^T, W [E, OUT, IN].
@@ -106,15 +115,16 @@ enum {
  * group_size 64, IN % 64 == 0, OUT % 16 == 0. VQ_REF: dim 2, 4 or 8,
  * K <= 65536, group_size a multiple of dim dividing IN, IN % 64 == 0,
  * OUT % 16 == 0. AFFINE (QuantizedSwitchLinear): bits 2, 3, 4, 5, 6 or 8,
- * group_size 32, 64 or 128, IN % 64 == 0, OUT % 16 == 0. A SwitchGLU's
- * three linears share one of VQ_REF and AFFINE, or use neither.
+ * group_size 32, 64 or 128, IN % 64 == 0, OUT % 16 == 0. FP8_BLOCK:
+ * group_size 128, IN % 16 == 0, OUT % 16 == 0. A SwitchGLU's three linears
+ * share one of VQ_REF, AFFINE and FP8_BLOCK, or use none of them.
  * Dense: IN % 16 == 0, OUT % 16 == 0. Pointers 16-byte aligned. */
 typedef struct {
     int32_t format;
     int32_t num_experts;
     int32_t out_features;
     int32_t in_features;
-    const void *weight;          /* DENSE_BF16 */
+    const void *weight;          /* DENSE_BF16, FP8_BLOCK, AFFINE (packed) */
     const void *codes;           /* VQ_U8 (device layout) */
     const void *codebook;        /* VQ_U8 */
     const void *scales;          /* VQ_U8 */
@@ -447,6 +457,29 @@ VQMOE_API vqmoe_status vqmoe_workspace_status(const void *workspace, void *strea
 VQMOE_API const char *vqmoe_last_error(void);
 
 VQMOE_API int32_t vqmoe_abi_version(void);
+
+/* x [rows, cols] bf16 (rows at a pitch of x_stride elements) -> q [rows, cols]
+ * e4m3 and scales [rows, ceil(cols/128)] float32. A row's group of 128 inputs
+ * (the last one ragged) with the largest magnitude a, at least 2^-100:
+ *   scale = f32(a / 448),  q = e4m3(448 x / a)   (the exact quotient, rounded
+ * once to nearest even). A NaN or an infinity in a group makes its scale NaN.
+ * cols % 16 == 0, x_stride % 8 == 0; x and q 16-byte aligned. */
+VQMOE_API vqmoe_status vqmoe_quantize_fp8(const void *x, int64_t rows, int32_t cols, int64_t x_stride, void *q,
+                                          float *scales, void *stream);
+
+/* Rows in group order times their group's weights: out[r] = x[r] @ W[e]^T for
+ * offsets[e] <= r < offsets[e+1] (device int32 [E+1], ascending; values
+ * outside [0, rows] are clamped). w: DENSE_BF16 or FP8_BLOCK, E <= 1024; with
+ * FP8_BLOCK the rows are quantized as vqmoe_quantize_fp8 does, into the
+ * workspace. offsets null: one group of all rows (E == 1), a dense linear.
+ * Rows of out that lie in no group are left as they were. x bf16, rows at a
+ * pitch of x_stride elements (a multiple of 8); out [rows, OUT] bf16 or float32
+ * (out_dtype), float32 sums rounded once. status (optional): a device word
+ * that a bounded wait raises when it runs out; the call never clears it. */
+VQMOE_API size_t vqmoe_grouped_linear_workspace_size(const vqmoe_linear *w, int32_t rows);
+VQMOE_API vqmoe_status vqmoe_grouped_linear(const vqmoe_linear *w, const void *x, int32_t rows, int64_t x_stride,
+                                            const int32_t *offsets, void *out, int32_t out_dtype, void *workspace,
+                                            size_t workspace_bytes, uint32_t *status, void *stream);
 
 #ifdef __cplusplus
 }

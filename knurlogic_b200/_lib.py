@@ -18,6 +18,7 @@ FMT_DENSE_BF16 = 0
 FMT_VQ_U8 = 1
 FMT_VQ_REF = 2          # reference-layout codes (uint8 / uint16), dim 2, 4 or 8
 FMT_AFFINE = 3          # affine-quantized (QuantizedSwitchLinear): packed q, scales, biases
+FMT_FP8_BLOCK = 4       # block-scaled e4m3 (Fp8Linear, Fp8SwitchLinear): weight, scales
 OUT_BF16 = 0
 OUT_F32 = 1
 ACT_SWIGLU = 0          # vqmoe_linear.activation of a SwitchGLU's gate linear
@@ -106,6 +107,11 @@ SIGNATURES = [
     ("vqmoe_moe_experts", c_int32,
      [POINTER(Linear), POINTER(Linear), POINTER(Linear), c_void_p, c_void_p, c_void_p, c_int32, c_int32,
       c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("vqmoe_quantize_fp8", c_int32, [c_void_p, c_int64, c_int32, c_int64, c_void_p, c_void_p, c_void_p]),
+    ("vqmoe_grouped_linear_workspace_size", c_size_t, [POINTER(Linear), c_int32]),
+    ("vqmoe_grouped_linear", c_int32,
+     [POINTER(Linear), c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_size_t, c_void_p,
+      c_void_p]),
     ("vqmoe_dequant", c_int32,
      [POINTER(Linear), c_int32, c_int32, c_void_p, c_void_p]),
     ("vqmoe_vq_layout_bytes", c_int32,

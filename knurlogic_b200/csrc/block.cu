@@ -129,7 +129,7 @@ combine_kernel(const uint16_t *__restrict__ ybuf, int T, int k, int H,
 
 static bool aligned_ptr(const void *p) { return p && aligned16(p); }
 
-static vqmoe_status check_linear(const vqmoe_linear *w, const char *name) {
+vqmoe_status check_linear(const vqmoe_linear *w, const char *name) {
     if (!w) return set_error(VQMOE_BAD_POINTER, "%s: null descriptor", name);
     if (w->num_experts <= 0 || w->out_features <= 0 || w->in_features <= 0)
         return set_error(VQMOE_BAD_SHAPE, "%s: non-positive shape", name);
@@ -142,6 +142,15 @@ static vqmoe_status check_linear(const vqmoe_linear *w, const char *name) {
                              w->in_features);
         if (!w->weight || !aligned16(w->weight))
             return set_error(VQMOE_BAD_POINTER, "%s: weight null or not 16-byte aligned", name);
+        return VQMOE_OK;
+    }
+    if (w->format == VQMOE_FMT_FP8_BLOCK) {
+        if (w->in_features % 16)
+            return set_error(VQMOE_BAD_SHAPE, "%s: in_features %d is not a multiple of 16", name, w->in_features);
+        if (w->group_size != 128)
+            return set_error(VQMOE_BAD_FORMAT, "%s: e4m3 scale blocks of %d (128)", name, w->group_size);
+        if (!aligned_ptr(w->weight) || !aligned_ptr(w->scales))
+            return set_error(VQMOE_BAD_POINTER, "%s: weight/scales null or not 16-byte aligned", name);
         return VQMOE_OK;
     }
     if (w->format == VQMOE_FMT_AFFINE) {
@@ -191,12 +200,15 @@ static vqmoe_status check_linear(const vqmoe_linear *w, const char *name) {
 }
 
 // a SwitchGLU's linears share one general-kernel format (reference-layout
-// VQ or affine) or use none
+// VQ or affine), are all block-scaled e4m3, or use none of these
 static vqmoe_status check_glu_formats(const vqmoe_linear *g, const vqmoe_linear *u, const vqmoe_linear *d) {
     if ((is_general(g->format) || is_general(u->format) || is_general(d->format)) &&
         (g->format != u->format || g->format != d->format))
         return set_error(VQMOE_BAD_FORMAT,
                          "gate/up/down: reference-layout VQ or affine on some linears but not all");
+    if ((is_fp8(g->format) || is_fp8(u->format) || is_fp8(d->format)) &&
+        (g->format != u->format || g->format != d->format))
+        return set_error(VQMOE_BAD_FORMAT, "gate/up/down: block-scaled e4m3 on some linears but not all");
     return VQMOE_OK;
 }
 
@@ -266,6 +278,7 @@ struct BlockWs {
     uint16_t *ybuf;
     uint16_t *sh;
     uint16_t *xs;        // the prefill path's expert-ordered inputs, or null
+    uint8_t *xq;         // e4m3 experts: the quantized inputs in expert order, or null
     size_t bytes;
 };
 
@@ -288,6 +301,7 @@ static BlockWs carve_block(void *ws, const vqmoe_block *b, int T) {
     w.sh = c.take<uint16_t>((size_t)T * H);
     const bool vq = b->gate.format == VQMOE_FMT_VQ_U8 && b->down.format == VQMOE_FMT_VQ_U8;
     w.xs = prefill_regime(vq, E, P) ? c.take<uint16_t>((size_t)P * H) : nullptr;
+    w.xq = is_fp8(b->gate.format) ? c.take<uint8_t>(fp8_rows_bytes(P, H)) : nullptr;
     w.bytes = align_up(c.off, 256);
     return w;
 }
@@ -371,6 +385,7 @@ static RoutedIO routed_io(const RouteWs &rt, int E, int k, int P, const void *x,
     r.out = out;
     r.out_f16 = out_f16;
     r.pair_scale = scale;
+    r.rank = rt.rank;
     return r;
 }
 
@@ -537,6 +552,8 @@ static vqmoe_status run_block(const vqmoe_block *b, const uint16_t *x, int T,
                             vq_dn, nullptr);
     r1.xs = w.xs;
     r1.act = b->gate.activation;
+    r1.inds = w.inds;
+    r1.xq = w.xq;
     // the expert split: the owned pairs' outputs go straight into this
     // rank's buffer, where the other ranks read them
     uint16_t *ybuf = tp && tp->ep_local ? reinterpret_cast<uint16_t *>(tp->base[tp->rank] + kTpFlagBytes) : w.ybuf;
@@ -578,6 +595,7 @@ struct GluWs {
     RouteWs rt;
     uint16_t *act;
     uint16_t *xs;        // the prefill path's expert-ordered inputs, or null
+    uint8_t *xq;         // e4m3 experts: the quantized inputs in expert order, or null
     size_t bytes;
 };
 
@@ -595,6 +613,7 @@ static GluWs carve_glu(void *ws, const vqmoe_linear *first, const vqmoe_linear *
     w.act = dual ? c.take<uint16_t>((size_t)P * I) : nullptr;
     const bool vq = first->format == VQMOE_FMT_VQ_U8 && (!dual || down->format == VQMOE_FMT_VQ_U8);
     w.xs = prefill_regime(vq, E, P) ? c.take<uint16_t>((size_t)P * H) : nullptr;
+    w.xq = is_fp8(first->format) ? c.take<uint8_t>(fp8_rows_bytes(P, H)) : nullptr;
     w.bytes = align_up(c.off, 256);
     return w;
 }
@@ -856,6 +875,8 @@ vqmoe_status vqmoe_switch_glu(const vqmoe_linear *gate, const vqmoe_linear *up,
                                 w.act, vq_dn, nullptr);
         r1.xs = w.xs;
         r1.act = gate->activation;
+        r1.inds = ind;
+        r1.xq = w.xq;
         RoutedIO r2 = routed_io(rt, E, top_k, P, w.act, 1,
                                 static_cast<uint16_t *>(y) + (size_t)t0 * top_k * H, 0, nullptr);
         if ((s = launch_experts(gate, up, &r1, down, r2, rt.zero, w.status, 0, st)) != VQMOE_OK) return s;
@@ -918,6 +939,8 @@ vqmoe_status vqmoe_moe_experts(const vqmoe_linear *gate, const vqmoe_linear *up,
                                 w.act, vq_dn, nullptr);
         r1.xs = w.xs;
         r1.act = gate->activation;
+        r1.inds = ind;
+        r1.xq = w.xq;
         RoutedIO r2 = routed_io(rt, E, top_k, P, w.act, 1, ybuf, 0, scores + (size_t)t0 * top_k);
         if ((s = launch_experts(gate, up, &r1, down, r2, rt.zero, w.status, 0, st)) != VQMOE_OK) return s;
         const size_t nvec = (size_t)T * (H / 8);
@@ -961,6 +984,8 @@ vqmoe_status vqmoe_switch_linear(const vqmoe_linear *w, const void *x, int32_t x
                                x_per_pair, static_cast<uint16_t *>(y) + (size_t)t0 * top_k * w->out_features,
                                0, nullptr);
         r.xs = ws.xs;
+        r.inds = indices + (size_t)t0 * top_k;
+        r.xq = ws.xq;
         if ((s = launch_experts(nullptr, nullptr, nullptr, w, r, rt.zero, ws.status, 0, st)) != VQMOE_OK) return s;
     }
     return VQMOE_OK;

@@ -199,6 +199,8 @@ inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 inline bool is_vq(int format) { return format == VQMOE_FMT_VQ_U8 || format == VQMOE_FMT_VQ_REF; }
 // a format the general (dequantise-into-shared-memory) expert kernel serves
 inline bool is_general(int format) { return format == VQMOE_FMT_VQ_REF || format == VQMOE_FMT_AFFINE; }
+// block-scaled e4m3 experts (gmm.cu)
+inline bool is_fp8(int format) { return format == VQMOE_FMT_FP8_BLOCK; }
 inline bool aligned16(const void *p) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }

@@ -238,16 +238,23 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-bool make_tma_map(CUtensorMap *m, const void *base, int rows, int cols, int box_rows) {
+// Row-major 2-D tensor, rows at a pitch of `pitch` bytes, 128-byte swizzled
+// boxes; out-of-range elements read as zero.
+CUresult encode_tma_2d(CUtensorMap *m, CUtensorMapDataType type, const void *base, const cuuint64_t (&dims)[2],
+                       cuuint64_t pitch, const cuuint32_t (&box)[2]) {
     auto fn = encode_fn();
-    if (!fn || rows <= 0 || cols <= 0 || (cols * 2) % 16 || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    if (!fn) return CUDA_ERROR_NOT_FOUND;
+    const cuuint64_t strides[1] = {pitch};
     const cuuint32_t es[2] = {1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return fn(m, type, 2, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+bool make_tma_map(CUtensorMap *m, const void *base, int rows, int cols, int box_rows) {
+    if (rows <= 0 || cols <= 0 || (cols * 2) % 16 || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    return encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, dims, (cuuint64_t)cols * 2, box) == CUDA_SUCCESS;
 }
 
 // The shared expert's dense matmul (+ SwiGLU when w1 is set) for many tokens

@@ -44,6 +44,8 @@ struct RoutedIO {
     const float *pair_scale;
     int act;                // a gate/up stage's VQMOE_ACT_*
     void *xs;               // [P][IN] fp16 scratch (the prefill path's sorted inputs), or null
+    const int32_t *inds, *rank;  // per pair: its expert, its place among the expert's pairs (-1: no such expert)
+    void *xq;               // e4m3 experts: the quantized inputs in expert order (fp8_rows_bytes), or null
 };
 
 // The prefill path (tcgen05 grouped GEMM) serves a call with VQ experts and
@@ -100,6 +102,12 @@ vqmoe_status launch_tp_gather(void *const *arrays, const int *widths, int T, int
 // phase 1 (r1, may be null) then phase 2, two launches.
 vqmoe_status launch_experts_ref(const vqmoe_linear *gate, const vqmoe_linear *up, const RoutedIO *r1,
                                 const vqmoe_linear *w2, const RoutedIO &r2, cudaStream_t stream);
+// The routed experts with block-scaled e4m3 weights (VQMOE_FMT_FP8_BLOCK).
+vqmoe_status launch_experts_fp8(const vqmoe_linear *gate, const vqmoe_linear *up, const RoutedIO *r1,
+                                const vqmoe_linear *w2, const RoutedIO &r2, uint32_t *err, cudaStream_t stream,
+                                cudaEvent_t after_permute);
+size_t fp8_rows_bytes(int rows, int in);
+vqmoe_status check_linear(const vqmoe_linear *w, const char *name);
 // The shared expert's dense matmul (+ SwiGLU when w1 is set): K slicing,
 // its partial buffer [ks][T][nmat][OUT] float and [ceil(OUT/32)] semaphores.
 void plan_shared_dense(int IN, int OUT, int nmat, int *ks, int *kslice, size_t *smem);

@@ -25,7 +25,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .switch_layers import (QuantizedSwitchLinear, SwitchGLU, SwitchLinear, VQSwitchLinear, c_stream,
+from .switch_layers import (Fp8SwitchLinear, QuantizedSwitchLinear, SwitchGLU, SwitchLinear, VQSwitchLinear, c_stream,
                             require_cuda)
 
 
@@ -233,7 +233,8 @@ class SparseMoeBlock(nn.Module):
         `{prefix}gate.weight`; `{prefix}switch_mlp.{gate,up,down}_proj.`
         `{codes, codebook, vq_scales}` (VQ), `{weight, scales, biases}`
         (affine-quantized; `group_size` default 64, `bits` from the packed
-        width) or `.weight` (bf16), or the HF
+        width), `{weight, weight_scale_inv}` (block-scaled e4m3) or
+        `.weight` (bf16), or the HF
         fused `{prefix}experts.gate_up_proj [E, 2I, H]` /
         `{prefix}experts.down_proj [E, H, I]` (split as
         `qwen3_5_moe.py:36-50`); `{prefix}shared_expert.{gate,up,down}_proj.`
@@ -264,6 +265,8 @@ class SparseMoeBlock(nn.Module):
                     gs = group_size or 64
                     nbits = bits or (wt.shape[-1] * 32) // (sc.shape[-1] * gs)
                     projs[n] = QuantizedSwitchLinear(wt, sc, w[q + "biases"], group_size=gs, bits=nbits)
+                elif q + "weight_scale_inv" in w:
+                    projs[n] = Fp8SwitchLinear(w[q + "weight"], w[q + "weight_scale_inv"])
                 elif q + "weight" in w:
                     projs[n] = SwitchLinear(w[q + "weight"])
                 else:

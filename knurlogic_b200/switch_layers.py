@@ -11,6 +11,8 @@ Reference interfaces mirrored here:
 * `SwitchLinear(weight)` -- mlx-lm's bf16 expert linear
   (`glm5_next/_mlx_vlm/models/switch_layers.py:89-125`).
 * `SwitchGLU(gate_proj, up_proj, down_proj)` -- `switch_layers.py:151-193`.
+`Fp8SwitchLinear` (block-scaled e4m3 experts) has the same call form and no
+counterpart in the reference.
 
 Every call runs on the CUDA path; there is no CPU implementation.
 """
@@ -351,6 +353,57 @@ class QuantizedSwitchLinear(_SwitchBase):
         d = self.descriptor()
         _lib.call("vqmoe_dequant", ctypes_ref(d), first, count, out.data_ptr(), _stream(out))
         return out
+
+
+def check_fp8_weight(weight: torch.Tensor, scales: torch.Tensor, dims: int) -> None:
+    """Block-scaled e4m3 weights [.., OUT, IN] (`dims` dimensions) with one
+    scale for each 128 x 128 block."""
+    want = "[E, OUT, IN]" if dims == 3 else "[OUT, IN]"
+    if weight.dim() != dims or weight.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"weight must be {want} float8_e4m3fn, got {tuple(weight.shape)} {weight.dtype}")
+    *lead, out, inp = weight.shape
+    if 0 in weight.shape or out % 16 or inp % 16:
+        raise ValueError(f"weight {tuple(weight.shape)}: OUT and IN must be multiples of 16")
+    shape = (*lead, -(-out // 128), -(-inp // 128))
+    if tuple(scales.shape) != shape:
+        raise ValueError(f"weight_scale_inv {tuple(scales.shape)}: one scale for each 128 x 128 block of "
+                         f"{tuple(weight.shape)} is {shape}")
+
+
+class Fp8SwitchLinear(_SwitchBase):
+    """Block-scaled e4m3 experts, as block-quantized checkpoints store them:
+    `weight [E, OUT, IN]` float8_e4m3fn and `weight_scale_inv [E,
+    ceil(OUT/128), ceil(IN/128)]` float32 (the factor that restores a block;
+    bf16 scales are widened). OUT and IN are multiples of 16.
+
+    The bf16 inputs are quantized on the way in (`quantize_fp8`: e4m3 with a
+    float32 scale for each row and 128 inputs), the products are summed in
+    float32 and the output rounded once to bf16. In a `SwitchGLU` the
+    activations between gate/up and down are quantized the same way."""
+
+    def __init__(self, weight: torch.Tensor, weight_scale_inv: torch.Tensor):
+        super().__init__()
+        check_fp8_weight(weight, weight_scale_inv, 3)
+        self.register_buffer("weight", weight.contiguous())
+        self.register_buffer("weight_scale_inv", weight_scale_inv.to(torch.float32).contiguous())
+
+    @property
+    def num_experts(self):
+        return self.weight.shape[0]
+
+    @property
+    def output_dims(self):
+        return self.weight.shape[1]
+
+    @property
+    def input_dims(self):
+        return self.weight.shape[2]
+
+    def descriptor(self) -> _lib.Linear:
+        require_cuda(self.weight, self.weight_scale_inv)
+        return _lib.Linear(format=_lib.FMT_FP8_BLOCK, num_experts=self.num_experts,
+                           out_features=self.output_dims, in_features=self.input_dims,
+                           weight=self.weight.data_ptr(), scales=self.weight_scale_inv.data_ptr(), group_size=128)
 
 
 class SwiGLU(nn.Module):

@@ -44,7 +44,7 @@ class MoEConfig:
     dim: int = 4
     codebook_size: int = 256
     group: int = 64
-    quant: str = "vq"           # vq | affine (mlx's weight / scales / biases)
+    quant: str = "vq"           # vq | affine (mlx's weight / scales / biases) | fp8 (block-scaled e4m3)
     bits: int = 4               # affine bits per weight
 
     def with_tokens(self, t: int) -> "MoEConfig":
@@ -105,6 +105,14 @@ def _affine_matrix(E, out, inp, cfg: MoEConfig, g: torch.Generator, device) -> d
     return {"weight": pack_affine(q, cfg.bits), "scales": s.to(torch.bfloat16), "biases": b.to(torch.bfloat16)}
 
 
+def _fp8_matrix(E, out, inp, g: torch.Generator, device) -> dict:
+    """e4m3 values near the type's range and a float32 scale for each 128 x
+    128 block (weights about N(0, 0.02)-sized)."""
+    w = (torch.randn((E, out, inp), generator=g, device=device) * 110.0).clamp_(-448.0, 448.0)
+    s = (0.7 + 0.6 * torch.rand((E, -(-out // 128), -(-inp // 128)), generator=g, device=device)) * (0.02 / 110.0)
+    return {"weight": w.to(torch.float8_e4m3fn), "weight_scale_inv": s}
+
+
 def make_weights(cfg: MoEConfig, seed: int = 0, device="cpu",
                  scales: str = "ones", prefix: str = "mlp.") -> dict:
     """State dict with the reference's names (reference layout for codes)."""
@@ -123,6 +131,10 @@ def make_weights(cfg: MoEConfig, seed: int = 0, device="cpu",
         q = f"{prefix}switch_mlp.{name}."
         if cfg.quant == "affine":
             for leaf, t in _affine_matrix(E, out, inp, cfg, g, device).items():
+                w[q + leaf] = t
+            continue
+        if cfg.quant == "fp8":
+            for leaf, t in _fp8_matrix(E, out, inp, g, device).items():
                 w[q + leaf] = t
             continue
         if cfg.codebook_size <= 256:
