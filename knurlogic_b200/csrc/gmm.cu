@@ -28,6 +28,9 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cstdlib>
+#include <map>
+#include <mutex>
 
 #include "experts.cuh"
 #include "gmm.cuh"
@@ -113,6 +116,20 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *v) {
         : "memory");
 }
 
+// One lane of the (converged) warp. The roles that issue copies and MMAs run
+// their loops with the whole warp and elect a lane for the issue alone: the
+// loop stays uniform, so descriptors and barriers are built in uniform
+// registers (an MMA a lane issues from a divergent loop took 92 cycles to
+// issue, 58 so: four a block, more than 128 x 16 of them need).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(threads) : "memory");
 }
@@ -291,8 +308,7 @@ __global__ void __launch_bounds__(kNThreads)
     if (weights_first && warp == 0) {
         const int dense_tiles = ((a.P + BN - 1) / BN) * ntiles;
         if (first < dense_tiles) early = min(C::kStages, kb1 - kb0);
-        __syncwarp();
-        if (lane == 0) {
+        if (elect_one()) {
             const int n0 = (first % ntiles) * kLanes;
             for (int s = 0; s < early; ++s) {
                 const uint32_t st = sbase + s * C::kStageBytes;
@@ -301,6 +317,7 @@ __global__ void __launch_bounds__(kNThreads)
                 if (GLU) tma_load_2d(st + kTileBytes, &tw1, (kb0 + s) * 128, n0, &full[s]);
             }
         }
+        __syncwarp();
     }
     pdl_wait();
     pdl_trigger();
@@ -312,38 +329,43 @@ __global__ void __launch_bounds__(kNThreads)
     const int tiles = (a.off ? s_g.pre[a.E] : (a.P + BN - 1) / BN) * ntiles;
     if (warp == 0) {
         // ---- TMA producer
-        if (lane == 0) {
-            uint32_t it = 0;
-            for (int tile = first; tile < tiles; tile += step) {
-                const Tile t = locate(a, s_g, tile, ntiles, BN);
-                const int wrow = t.e * a.N + t.nt * kLanes;
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % C::kStages;
-                    const uint32_t st = sbase + s * C::kStageBytes;
-                    if (it >= (uint32_t)early) {
-                        if (it >= (uint32_t)C::kStages) wait(&empty[s], ((it / C::kStages) + 1) & 1);
+        int s = 0;
+        uint32_t phase = 1;                         // an empty stage's first wait passes
+        for (int tile = first; tile < tiles; tile += step) {
+            const Tile t = locate(a, s_g, tile, ntiles, BN);
+            const int wrow = t.e * a.N + t.nt * kLanes;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const uint32_t st = sbase + s * C::kStageBytes;
+                wait(&empty[s], phase);
+                if (elect_one()) {
+                    if (early <= 0) {
                         arrive_expect_tx(&full[s], C::kStageBytes);
                         tma_load_2d(st, &tw0, kb * 128, wrow, &full[s]);
                         if (GLU) tma_load_2d(st + kTileBytes, &tw1, kb * 128, wrow, &full[s]);
                     }
                     tma_load_2d(st + NMAT * kTileBytes, &tx, kb * 128, t.row0, &full[s]);
                 }
+                __syncwarp();
+                --early;
+                if (++s == C::kStages) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
         }
     } else if (warp == 1) {
         // ---- MMA issuer: one accumulator a scale block (e4m3) or a tile (bf16)
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_of(FP8, BN);
-            uint32_t it = 0, un = 0;
-            for (int tile = first; tile < tiles; tile += step) {
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const bool fresh = FP8 || kb == kb0, last = FP8 || kb == kb1 - 1;
-                    const uint32_t u = un % C::kUnits;
-                    if (fresh && un >= (uint32_t)C::kUnits) wait(&acc_empty[u], ((un / C::kUnits) + 1) & 1);
-                    const int s = it % C::kStages;
-                    wait(&full[s], (it / C::kStages) & 1);
-                    tc_fence_after();
-                    const uint32_t st = sbase + s * C::kStageBytes, d = tmem + u * C::kCols;
+        constexpr uint32_t idesc = idesc_of(FP8, BN);
+        int s = 0, u = 0;
+        uint32_t phase = 0, uphase = 1;
+        for (int tile = first; tile < tiles; tile += step) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const bool fresh = FP8 || kb == kb0, last = FP8 || kb == kb1 - 1;
+                if (fresh) wait(&acc_empty[u], uphase);
+                wait(&full[s], phase);
+                tc_fence_after();
+                const uint32_t st = sbase + s * C::kStageBytes, d = tmem + u * C::kCols;
+                if (elect_one()) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -351,14 +373,19 @@ __global__ void __launch_bounds__(kNThreads)
                             mma_ss<FP8>(d + m * BN, sw128_desc(st + m * kTileBytes + 32 * q),
                                         sw128_desc(st + NMAT * kTileBytes + 32 * q), idesc, !fresh || q > 0);
                     tc_commit(&empty[s]);
-                    if (last) {
-                        tc_commit(&acc_full[u]);
-                        ++un;
-                    }
+                    if (last) tc_commit(&acc_full[u]);
+                }
+                __syncwarp();
+                if (++s == C::kStages) {
+                    s = 0;
+                    phase ^= 1;
+                }
+                if (last && ++u == C::kUnits) {
+                    u = 0;
+                    uphase ^= 1;
                 }
             }
         }
-        __syncwarp();
     } else {
         // ---- epilogue: thread = one weight row, warp w the TMEM lanes 32 (w % 4) ..
         const int q = warp & 3, row = 32 * q + lane, et = tid - 64;
@@ -400,8 +427,7 @@ __global__ void __launch_bounds__(kNThreads)
                 }
                 const float f0 = FP8 ? __ldg(w0 + kb0 + i) : 1.0f, f1 = FP8 && GLU ? __ldg(w1 + kb0 + i) : 1.0f;
                 const uint32_t u = un % C::kUnits;
-                if (lane == 0) wait(&acc_full[u], (un / C::kUnits) & 1);
-                __syncwarp();
+                wait(&acc_full[u], (un / C::kUnits) & 1);
                 tc_fence_after();
                 constexpr int kStep = BN < 32 ? 16 : 32;
 #pragma unroll
@@ -568,6 +594,15 @@ constexpr int kMStages = 4;
 constexpr int kMStageBytes = kTileBytes + kCols * 128;
 constexpr size_t kMSmem = 1024 + (size_t)kMStages * kMStageBytes;
 constexpr int kMThreads = 384;                 // TMA, MMA, two idle warps, eight epilogue warps
+constexpr int kCtlRegs = 40, kEpiRegs = 232;   // setmaxnreg: 128 x 40 + 256 x 232 = 384 x 168
+
+// SwiGLU / GeGLU of two columns, every step rounded to bf16: packed bf16
+__device__ __forceinline__ uint32_t glu_pair(float g0, float g1, float u0, float u1, int act) {
+    const uint32_t g = cvt_bf16x2(g0, g1), u = cvt_bf16x2(u0, u1);
+    const uint32_t a = act == VQMOE_ACT_GEGLU ? cvt_bf16x2(gelu_tanh_f32(bf_lo(g)), gelu_tanh_f32(bf_hi(g)))
+                                              : cvt_bf16x2(silu_fast(bf_lo(g)), silu_fast(bf_hi(g)));
+    return cvt_bf16x2(bf_lo(a) * bf_lo(u), bf_hi(a) * bf_hi(u));
+}
 
 template <bool GLU, bool FP8>
 __global__ void __launch_bounds__(kMThreads, 1)
@@ -609,122 +644,136 @@ __global__ void __launch_bounds__(kMThreads, 1)
     const int tiles = (a.off ? s_g.pre[a.E] : (a.P + kLanes - 1) / kLanes) * ntiles;
     Waiter wait{a.err};
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
-        if (warp == 0 && lane == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kCtlRegs));
+        if (warp == 0) {
             // ---- TMA producer
-            uint32_t it = 0;
+            int s = 0;
+            uint32_t phase = 1;
             for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
                 const Tile t = locate(a, s_g, tile, ntiles, kLanes);
                 const int wrow = t.e * a.N + t.nt * kOutCols;
-                for (int kb = 0; kb < a.KB; ++kb, ++it) {
-                    const int s = it % kMStages;
+                for (int kb = 0; kb < a.KB; ++kb) {
                     const uint32_t st = sbase + s * kMStageBytes;
-                    if (it >= (uint32_t)kMStages) wait(&empty[s], ((it / kMStages) + 1) & 1);
-                    arrive_expect_tx(&full[s], kMStageBytes);
-                    tma_load_2d(st, &tx, kb * 128, t.row0, &full[s]);
-                    tma_load_2d(st + kTileBytes, &tw0, kb * 128, wrow, &full[s]);
-                    if (GLU) tma_load_2d(st + 2 * kTileBytes, &tw1, kb * 128, wrow, &full[s]);
+                    wait(&empty[s], phase);
+                    if (elect_one()) {
+                        arrive_expect_tx(&full[s], kMStageBytes);
+                        tma_load_2d(st, &tx, kb * 128, t.row0, &full[s]);
+                        tma_load_2d(st + kTileBytes, &tw0, kb * 128, wrow, &full[s]);
+                        if (GLU) tma_load_2d(st + 2 * kTileBytes, &tw1, kb * 128, wrow, &full[s]);
+                    }
+                    __syncwarp();
+                    if (++s == kMStages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
             }
-        } else if (warp == 1 && lane == 0) {
-            // ---- MMA issuer
+        } else if (warp == 1) {
+            // ---- MMA issuer: one accumulator a scale block (e4m3) or a tile (bf16)
             constexpr uint32_t idesc = idesc_of(FP8, kCols);
-            uint32_t it = 0, un = 0;
+            int s = 0;
+            uint32_t phase = 0, u = 0, uphase = 1;
             for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                for (int kb = 0; kb < a.KB; ++kb, ++it) {
+                for (int kb = 0; kb < a.KB; ++kb) {
                     const bool fresh = FP8 || kb == 0, last = FP8 || kb == a.KB - 1;
-                    const uint32_t u = un & 1;
-                    if (fresh && un >= 2) wait(&acc_empty[u], ((un >> 1) + 1) & 1);
-                    const int s = it % kMStages;
-                    wait(&full[s], (it / kMStages) & 1);
+                    if (fresh) wait(&acc_empty[u], uphase);
+                    wait(&full[s], phase);
                     tc_fence_after();
-                    const uint32_t st = sbase + s * kMStageBytes;
+                    const uint32_t st = sbase + s * kMStageBytes, d = tmem + u * kCols;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        mma_ss<FP8>(tmem + u * kCols, sw128_desc(st + 32 * q), sw128_desc(st + kTileBytes + 32 * q),
-                                    idesc, !fresh || q > 0);
-                    tc_commit(&empty[s]);
+                        for (int q = 0; q < 4; ++q)
+                            mma_ss<FP8>(d, sw128_desc(st + 32 * q), sw128_desc(st + kTileBytes + 32 * q), idesc,
+                                        !fresh || q > 0);
+                        tc_commit(&empty[s]);
+                        if (last) tc_commit(&acc_full[u]);
+                    }
+                    __syncwarp();
+                    if (++s == kMStages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                     if (last) {
-                        tc_commit(&acc_full[u]);
-                        ++un;
+                        u ^= 1;
+                        if (u == 0) uphase ^= 1;
                     }
                 }
             }
         }
-        __syncwarp();
     } else {
-        // ---- epilogue: thread = one token, half of the tile's columns
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;\n");
+        // ---- epilogue: thread = one token, half of the tile's columns: 128
+        // weight rows, or (gate/up) 64 of each matrix
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpiRegs));
         const int q = warp & 3, half = (warp - 4) >> 2, row = 32 * q + lane;
         const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16);
+        // its accumulator columns in four pieces of 32
+        auto piece = [&](int c) -> uint32_t { return GLU ? 64 * half + (c & 1) * 32 + (c >> 1) * 128 : 128 * half + 32 * c; };
+        const int NB = (a.N + kScaleBlock - 1) / kScaleBlock;
         uint32_t un = 0;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
             const Tile t = locate(a, s_g, tile, ntiles, kLanes);
             const int r = t.row0 + row;
             const bool live = r < t.end;
-            // this thread's 128 accumulator columns, in four pieces of 32:
-            // columns 128 half .. of the tile, or (gate/up) 64 half .. of each matrix
-            const uint32_t c0 = GLU ? 64 * half : 128 * half;
-            auto piece = [&](int c) -> uint32_t { return GLU ? c0 + (c & 1) * 32 + (c >> 1) * 128 : c0 + c * 32; };
-            const int n0 = t.nt * kOutCols + c0;       // its first output column
+            const int n0 = t.nt * kOutCols + piece(0);   // its first output column
             float acc[128];
             const float *w0 = nullptr, *w1 = nullptr;
             if (FP8) {
 #pragma unroll
                 for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-                const int NB = (a.N + kScaleBlock - 1) / kScaleBlock;
                 const size_t at = ((size_t)t.e * NB + min(n0 / kScaleBlock, NB - 1)) * a.KB;
                 w0 = a.sw0 + at;
                 w1 = GLU ? a.sw1 + at : w0;
             }
             const int units = FP8 ? a.KB : 1;
             float sx = FP8 && live ? __ldg(a.sx + r) : 0.0f;
-            float f0 = FP8 ? __ldg(w0) : 1.0f, f1 = FP8 ? __ldg(w1) : 1.0f;
+            float f0 = FP8 ? __ldg(w0) : 1.0f, f1 = FP8 && GLU ? __ldg(w1) : 1.0f;
             for (int i = 0; i < units; ++i, ++un) {
-                const float s0 = sx * f0, s1 = sx * f1;
+                const float s0 = sx * f0, s1 = GLU ? sx * f1 : s0;
                 if (FP8 && i + 1 < units) {            // the next block's scales
                     if (live) sx = __ldg(a.sx + (size_t)(i + 1) * a.P + r);
                     f0 = __ldg(w0 + i + 1);
                     if (GLU) f1 = __ldg(w1 + i + 1);
-                    else f1 = f0;
                 }
-                const uint32_t u = un & 1;
-                if (lane == 0) wait(&acc_full[u], (un >> 1) & 1);
-                __syncwarp();
+                const uint32_t u = un & 1, td = tq + u * kCols;
+                wait(&acc_full[u], (un >> 1) & 1);
                 tc_fence_after();
+                uint32_t dv[2][32];
+                auto add = [&](int c) {
+                    const float s = c >= 2 ? s1 : s0;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t dv[32];
-                    tmem_ld32(tq + u * kCols + piece(c), dv);
-                    tmem_wait_ld();
-                    if (c == 3) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&acc_empty[u]);
+                    for (int j = 0; j < 32; j += 2) {
+                        if (FP8) {
+                            fma2(acc[32 * c + j], acc[32 * c + j + 1], dv[c & 1][j], dv[c & 1][j + 1], s, s);
+                        } else {
+                            acc[32 * c + j] = __uint_as_float(dv[c & 1][j]);
+                            acc[32 * c + j + 1] = __uint_as_float(dv[c & 1][j + 1]);
+                        }
                     }
-                    if (FP8) {
-                        const float s = GLU && c >= 2 ? s1 : s0;
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2)
-                            fma2(acc[32 * c + j], acc[32 * c + j + 1], dv[j], dv[j + 1], s, s);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) acc[32 * c + j] = __uint_as_float(dv[j]);
-                    }
-                }
+                };
+                tmem_ld32(td + piece(0), dv[0]);
+                tmem_ld32(td + piece(1), dv[1]);
+                tmem_wait_ld();
+                add(0);
+                tmem_ld32(td + piece(2), dv[0]);
+                add(1);
+                tmem_ld32(td + piece(3), dv[1]);
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[u]);
+                add(2);
+                add(3);
             }
             if (GLU) {
                 // 64 activations of the token's group of 128; the largest of
                 // all 128 with the other half's warp
-                uint32_t m = 0;
-                uint32_t v[32];
+                uint32_t m = 0, v[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
-                    const uint32_t lo = __float_as_uint(glu_value(acc[2 * j], acc[64 + 2 * j], a.act)) >> 16;
-                    const uint32_t hi = __float_as_uint(glu_value(acc[2 * j + 1], acc[64 + 2 * j + 1], a.act)) >> 16;
-                    v[j] = lo | (hi << 16);
-                    if (n0 + 2 * j < a.N) m = max(m, max(lo & 0x7FFFu, hi & 0x7FFFu));
+                    v[j] = glu_pair(acc[2 * j], acc[2 * j + 1], acc[64 + 2 * j], acc[65 + 2 * j], a.act);
+                    if (n0 + 2 * j < a.N) m = __vmaxu2(m, v[j] & 0x7FFF7FFFu);
                 }
+                m = max(m & 0xFFFFu, m >> 16);
                 s_amax[half * kLanes + row] = m;
                 bar_sync(1, 256);
                 m = max(m, s_amax[(half ^ 1) * kLanes + row]);
@@ -781,14 +830,23 @@ __global__ void __launch_bounds__(kMThreads, 1)
 
 // ---------------------------------------------------------------- host
 
-// tok_m_kernel's epilogue warps take registers (setmaxnreg) that its other
-// warps gave up: 128 x 40 + 256 x 232 of the 384 x 168 it is launched with. A
-// build that launches with fewer would wait for them without end.
+// The epilogue warps take registers that the block's other warps gave up. A
+// build that launches with fewer than the two shares' sum would wait for them
+// without end: refused (looked up once per kernel and device).
 static vqmoe_status check_registers(const void *fn) {
-    cudaFuncAttributes at{};
-    if (cudaFuncGetAttributes(&at, fn) != cudaSuccess) return check_launch("tok_m_kernel");
-    if (at.numRegs * kMThreads < 128 * 40 + 256 * 232)
-        return set_error(VQMOE_LAUNCH_FAILED, "tok_m_kernel: built with %d registers a thread", at.numRegs);
+    static std::mutex mu;
+    static std::map<std::pair<const void *, int>, int> regs;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("tok_m_kernel");
+    std::lock_guard<std::mutex> lock(mu);
+    int &n = regs[{fn, dev}];
+    if (!n) {
+        cudaFuncAttributes at{};
+        if (cudaFuncGetAttributes(&at, fn) != cudaSuccess) return check_launch("tok_m_kernel");
+        n = at.numRegs;
+    }
+    if (n * kMThreads < 128 * kCtlRegs + 256 * kEpiRegs)
+        return set_error(VQMOE_LAUNCH_FAILED, "tok_m_kernel: built with %d registers a thread", n);
     return VQMOE_OK;
 }
 
@@ -853,9 +911,10 @@ vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const voi
     // groups that can have rows, and their mean rows
     const int groups = std::min(a.E, a.P), mean = (a.P + groups - 1) / groups;
     const int bn_max = glu ? 64 : 128;
+    const char *env = getenv("GMM_M"); const int thr = env ? atoi(env) : bn_max;
     Maps m;
     const size_t wrows = (size_t)a.E * a.N;
-    if (mean > bn_max) {
+    if (mean > thr) {
         if (!byte_map(&m.x, x, a.P, row_bytes, x_pitch, kLanes) ||
             !byte_map(&m.w0, w0, wrows, row_bytes, row_bytes, glu ? 128 : kCols) ||
             !byte_map(&m.w1, glu ? w1 : w0, wrows, row_bytes, row_bytes, 128))
