@@ -5,25 +5,29 @@
 //   y[r][n] = sum_b sx[b][r] sw[e][n / 128][b] (sum over block b of x w)
 // A block's inner sum is four tcgen05.mma of 32 inputs into TMEM; the scales
 // differ from block to block, so the epilogue warps read every block's sum
-// back and add it, scaled, to float32 registers, while the tensor core works
-// on the next blocks (TMEM holds two to four of them). bf16 needs none of
-// this: a tile's whole sum stays in TMEM.
+// back and add it, scaled, to float32 registers while the tensor core works
+// on the next blocks. bf16 needs none of this: a tile's whole sum stays in
+// TMEM.
 //
 // The groups' rows are contiguous (`off`, on the device): a tile is rows of
 // one group. Rows past the group's end that a TMA box brings along belong to
-// another group or are zero; they are lines of the product that are never
+// another group or are zero; they are lanes of the accumulator that are never
 // stored.
 //
-// Two kernels, by which operand takes the 128 lanes of the accumulator:
-//   tok_n_kernel  weight rows on the lanes, 16-128 tokens as the MMA's N:
-//                 few tokens a group. Bound by streaming the weights; with
-//                 few tiles a cluster of CTAs shares a tile's inputs and adds
-//                 its partial sums through distributed shared memory.
-//   tok_m_kernel  128 tokens on the lanes, 256 weight rows as N: many tokens a
-//                 group. Bound by the tensor cores and by feeding them.
-// Both run persistent CTAs of specialised warps: one issues TMA copies into a
-// ring of 128-byte-swizzled stages, one issues the MMAs, the others are the
-// epilogue.
+// A tile is up to 128 tokens (the accumulator's lanes, so that a thread's
+// token scale is one register) x 256 weight rows (gate/up: 128 of each), with
+// two TMEM buffers. Persistent CTAs of specialised warps: warp 0 issues TMA
+// copies of 128-byte rows into a ring of 128-byte-swizzled stages, warp 1
+// issues the MMAs, warps 4-7 and 8-11 are the epilogues of the accumulator's
+// two halves of 128 columns. Three modes:
+//   kPair    two CTAs (cta_group::2) share a tile of 256 tokens: each loads its
+//            128 tokens and half of the weight rows, so a block costs a CTA 32
+//            KB of L2 reads instead of 48. Many tokens a group.
+//   kSingle  one CTA a tile, fewer token rows loaded when groups are small: the
+//            weights' stream bounds it.
+//   kSplit   few tiles: a cluster of up to 8 CTAs shares a tile's blocks; the
+//            partial sums meet in distributed shared memory, added in rank
+//            order.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -44,18 +48,25 @@ namespace gm {
 using namespace tc;
 
 constexpr int kLanes = 128;                    // rows of an accumulator (MMA M)
-constexpr int kTileBytes = kLanes * 128;       // 128 rows x 128 bytes
-constexpr int kChunk = 16;                     // scale blocks staged at a time (tok_n)
 
-// A wait that ran out is recorded where the caller gave a word for it.
+// A whole warp's wait, first without the suspending form (a barrier that is
+// ready already costs the least so). One that ran out is recorded where the
+// caller gave a word for it, and every later one is skipped.
 struct Waiter {
     uint32_t *err;
     bool failed = false;
     __device__ void operator()(uint64_t *bar, uint32_t parity) {
-        if (failed) return;
         const uint32_t a = smem_u32(bar);
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(done)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (__all_sync(0xffffffffu, done) || failed) return;
         for (int i = 0; i < kPoll; ++i) {
-            uint32_t done;
             asm volatile(
                 "{\n\t.reg .pred p;\n\t"
                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -63,58 +74,86 @@ struct Waiter {
                 : "=r"(done)
                 : "r"(a), "r"(parity), "r"(kSuspendNs)
                 : "memory");
-            if (done) return;
+            if (__all_sync(0xffffffffu, done)) return;
         }
         failed = true;
         if (err) atomicExch(err, kWaitPipeline);
     }
 };
 
-template <bool FP8>
+// One 32-byte-deep MMA of this CTA (PAIR: of both CTAs, issued by the leader)
+template <bool FP8, bool PAIR>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
-    if (FP8)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-            "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-            "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
-            : "memory");
+#define VQMOE_MMA(GROUP, KIND)                                                                      \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                   \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), \
+                 "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)                                       \
+                 : "memory")
+    if (FP8 && PAIR) VQMOE_MMA("2", "f8f6f4");
+    else if (FP8) VQMOE_MMA("1", "f8f6f4");
+    else if (PAIR) VQMOE_MMA("2", "f16");
+    else VQMOE_MMA("1", "f16");
+#undef VQMOE_MMA
 }
 
 // D f32, A and B e4m3 (kind::f8f6f4) or bf16 (kind::f16), both K-major
-constexpr uint32_t idesc_of(bool fp8, int n) {
-    return (1u << 4) | (fp8 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(n >> 3) << 17) |
-           ((uint32_t)(kLanes >> 4) << 24);
+constexpr uint32_t idesc_of(bool fp8, int m, int n) {
+    return (1u << 4) | (fp8 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// d += s * v, two float32 at a time
-__device__ __forceinline__ void fma2(float &d0, float &d1, uint32_t v0, uint32_t v1, float s0, float s1) {
-    asm("{\n\t.reg .b64 a, b, c;\n\t"
-        "mov.b64 a, {%2, %3};\n\t"
-        "mov.b64 b, {%4, %5};\n\t"
-        "mov.b64 c, {%0, %1};\n\t"
-        "fma.rn.f32x2 c, a, b, c;\n\t"
-        "mov.b64 {%0, %1}, c;\n\t}\n"
-        : "+f"(d0), "+f"(d1)
-        : "f"(__uint_as_float(v0)), "f"(__uint_as_float(v1)), "f"(s0), "f"(s1));
+// The MMAs issued so far arrive on `bar` when they are done (PAIR: on both
+// CTAs' barrier at that place).
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    if (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(
+                smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        tc_commit(bar);
 }
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *v) {
+// An arrival on this CTA's barrier (PAIR: on the leader's)
+template <bool PAIR>
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .b32 r;\n\t"
+            "mapa.shared::cluster.u32 r, %0, 0;\n\t"
+            "mbarrier.arrive.shared::cluster.b64 _, [r];\n\t}\n" ::"r"(smem_u32(bar))
+            : "memory");
+    else
+        mbar_arrive(bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ bool rank_issues(int rank) {
+    return !PAIR || rank == 0;
+}
+// A copy of a pair's CTA into its own shared memory that counts on the
+// leader's barrier
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void *map, int c0, int c1, uint64_t *bar) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-        "%13, %14, %15}, [%16];\n"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr)
+        "{\n\t.reg .b32 r;\n\t"
+        "mapa.shared::cluster.u32 r, %2, 0;\n\t"
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%3, %4}], [r];\n\t}\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
         : "memory");
 }
+
+// Two float32 in a 64-bit register, as the packed multiply-add takes them: kept
+// packed throughout, so that no moves come between it and tcgen05.ld's registers
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ void fma2(uint64_t &d, uint64_t v, uint64_t s) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;\n" : "+l"(d) : "l"(v), "l"(s));
+}
+__device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
 // One lane of the (converged) warp. The roles that issue copies and MMAs run
 // their loops with the whole warp and elect a lane for the issue alone: the
@@ -136,11 +175,14 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 __device__ __forceinline__ void cluster_arrive_wait() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t saddr, uint32_t cta) {
+__device__ __forceinline__ uint32_t map_cluster(uint32_t saddr, int cta) {
     uint32_t r;
-    float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(saddr), "r"(cta));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(r) : "memory");
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
 
@@ -203,12 +245,6 @@ __device__ __forceinline__ Tile locate(const GmmArgs &a, const Groups &g, int ti
     return t;
 }
 
-// bf16(bf16(act(g)) * u), g and u the bf16 outputs of the gate and up products
-__device__ __forceinline__ float glu_value(float g, float u, int act) {
-    const float gb = bf16r(g);
-    return bf16r(bf16r(act == VQMOE_ACT_GEGLU ? gelu_tanh_f32(gb) : silu_f32(gb)) * bf16r(u));
-}
-
 // The quantizer's two numbers of a group whose largest |bf16| has the bits
 // `amax`: its scale f32(a / 448), and what quantize1() divides by. a is at
 // least 2^-100; a NaN or an infinity in the group makes the scale NaN.
@@ -240,361 +276,19 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
     return r;
 }
 
-// ------------------------------------------- few tokens: tokens as the MMA's N
+// ------------------------------------------------------------- the kernel
 
-template <int BN, int NMAT, bool FP8, bool SPLIT>
-struct NCfg {
-    static constexpr int kStageBytes = NMAT * kTileBytes + BN * 128;
-    static constexpr int kBudget = 196 * 1024;                     // one CTA an SM
-    static constexpr int kPartBytes = SPLIT ? NMAT * BN * kLanes * 4 : 0;
-    static constexpr int kOutBytes = BN * kLanes * 2;
-    static constexpr int kFit = (kBudget - kPartBytes - kOutBytes) / kStageBytes;
-    static constexpr int kStages = kFit > 12 ? 12 : kFit;
-    static constexpr int kCols = NMAT * BN;                        // one accumulator
-    static constexpr int kUnits = 512 / kCols > 4 ? 4 : 512 / kCols;
-    static constexpr int kWant = kUnits * kCols;
-    static constexpr int kAlloc = kWant <= 32 ? 32 : kWant <= 64 ? 64 : kWant <= 128 ? 128 : kWant <= 256 ? 256 : 512;
-    static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kPartBytes + kOutBytes;
-    static_assert(kStages >= 2 && kUnits >= 1, "tile too large");
-};
+enum Mode { kSingle = 0, kSplit = 1, kPair = 2 };
 
-constexpr int kNThreads = 192;
-
-template <int BN, int NMAT, bool FP8, bool SPLIT>
-__global__ void __launch_bounds__(kNThreads)
-    tok_n_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw0,
-                 const __grid_constant__ CUtensorMap tw1, const GmmArgs a, int weights_first) {
-    using C = NCfg<BN, NMAT, FP8, SPLIT>;
-    constexpr bool GLU = NMAT == 2;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[C::kStages], empty[C::kStages], acc_full[C::kUnits], acc_empty[C::kUnits];
-    __shared__ uint32_t s_tmem;
-    __shared__ Groups s_g;
-    __shared__ __align__(16) float s_sx[FP8 ? kChunk * BN : 1];
-    __shared__ float s_rs[BN];
-    __shared__ int s_row[BN];
-    __shared__ uint32_t s_amax[GLU ? BN : 1];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t *const sgen = smem_raw + (sbase - smem_u32(smem_raw));
-    float *const s_part = reinterpret_cast<float *>(sgen + C::kStages * C::kStageBytes);
-    uint16_t *const s_out = reinterpret_cast<uint16_t *>(sgen + C::kStages * C::kStageBytes + C::kPartBytes);
-    if (tid == 0) {
-        for (int i = 0; i < C::kStages; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-        }
-        for (int i = 0; i < C::kUnits; ++i) {
-            mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 4);
-        }
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)),
-                     "r"(C::kAlloc)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
-    }
-    const int ntiles = (a.N + kLanes - 1) / kLanes;
-    const int S = SPLIT ? a.split : 1, part = SPLIT ? blockIdx.x % S : 0;
-    const int first = blockIdx.x / S, step = gridDim.x / S;
-    const int kb0 = (int)((long long)a.KB * part / S), kb1 = (int)((long long)a.KB * (part + 1) / S);
-    Waiter wait{a.err};
-    // A dense product's weights do not depend on the kernel before this one:
-    // the first stages' weights are on their way before its result is waited
-    // for.
-    int early = 0;
-    if (weights_first && warp == 0) {
-        const int dense_tiles = ((a.P + BN - 1) / BN) * ntiles;
-        if (first < dense_tiles) early = min(C::kStages, kb1 - kb0);
-        if (elect_one()) {
-            const int n0 = (first % ntiles) * kLanes;
-            for (int s = 0; s < early; ++s) {
-                const uint32_t st = sbase + s * C::kStageBytes;
-                arrive_expect_tx(&full[s], C::kStageBytes);
-                tma_load_2d(st, &tw0, (kb0 + s) * 128, n0, &full[s]);
-                if (GLU) tma_load_2d(st + kTileBytes, &tw1, (kb0 + s) * 128, n0, &full[s]);
-            }
-        }
-        __syncwarp();
-    }
-    pdl_wait();
-    pdl_trigger();
-    if (a.off && warp == 0) build_groups(a, s_g, BN);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = s_tmem;
-    const int tiles = (a.off ? s_g.pre[a.E] : (a.P + BN - 1) / BN) * ntiles;
-    if (warp == 0) {
-        // ---- TMA producer
-        int s = 0;
-        uint32_t phase = 1;                         // an empty stage's first wait passes
-        for (int tile = first; tile < tiles; tile += step) {
-            const Tile t = locate(a, s_g, tile, ntiles, BN);
-            const int wrow = t.e * a.N + t.nt * kLanes;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const uint32_t st = sbase + s * C::kStageBytes;
-                wait(&empty[s], phase);
-                if (elect_one()) {
-                    if (early <= 0) {
-                        arrive_expect_tx(&full[s], C::kStageBytes);
-                        tma_load_2d(st, &tw0, kb * 128, wrow, &full[s]);
-                        if (GLU) tma_load_2d(st + kTileBytes, &tw1, kb * 128, wrow, &full[s]);
-                    }
-                    tma_load_2d(st + NMAT * kTileBytes, &tx, kb * 128, t.row0, &full[s]);
-                }
-                __syncwarp();
-                --early;
-                if (++s == C::kStages) {
-                    s = 0;
-                    phase ^= 1;
-                }
-            }
-        }
-    } else if (warp == 1) {
-        // ---- MMA issuer: one accumulator a scale block (e4m3) or a tile (bf16)
-        constexpr uint32_t idesc = idesc_of(FP8, BN);
-        int s = 0, u = 0;
-        uint32_t phase = 0, uphase = 1;
-        for (int tile = first; tile < tiles; tile += step) {
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const bool fresh = FP8 || kb == kb0, last = FP8 || kb == kb1 - 1;
-                if (fresh) wait(&acc_empty[u], uphase);
-                wait(&full[s], phase);
-                tc_fence_after();
-                const uint32_t st = sbase + s * C::kStageBytes, d = tmem + u * C::kCols;
-                if (elect_one()) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-#pragma unroll
-                        for (int m = 0; m < NMAT; ++m)
-                            mma_ss<FP8>(d + m * BN, sw128_desc(st + m * kTileBytes + 32 * q),
-                                        sw128_desc(st + NMAT * kTileBytes + 32 * q), idesc, !fresh || q > 0);
-                    tc_commit(&empty[s]);
-                    if (last) tc_commit(&acc_full[u]);
-                }
-                __syncwarp();
-                if (++s == C::kStages) {
-                    s = 0;
-                    phase ^= 1;
-                }
-                if (last && ++u == C::kUnits) {
-                    u = 0;
-                    uphase ^= 1;
-                }
-            }
-        }
-    } else {
-        // ---- epilogue: thread = one weight row, warp w the TMEM lanes 32 (w % 4) ..
-        const int q = warp & 3, row = 32 * q + lane, et = tid - 64;
-        uint32_t un = 0;
-        for (int tile = first; tile < tiles; tile += step) {
-            const Tile t = locate(a, s_g, tile, ntiles, BN);
-            const int np = min(BN, t.end - t.row0);
-            float acc[NMAT][BN];
-#pragma unroll
-            for (int m = 0; m < NMAT; ++m)
-#pragma unroll
-                for (int j = 0; j < BN; ++j) acc[m][j] = 0.0f;
-            bar_sync(1, 128);                       // the last tile's staging has been read
-            for (int j = et; j < BN; j += 128) {
-                const int r = t.row0 + j;
-                const int o = j < np ? (a.map ? a.map[r] : r) : -1;
-                s_row[j] = o;
-                s_rs[j] = a.row_scale && o >= 0 ? a.row_scale[o] : 1.0f;
-                if (GLU) s_amax[j] = 0;
-            }
-            const float *w0 = nullptr, *w1 = nullptr;
-            if (FP8) {
-                const size_t at = ((size_t)t.e * ntiles + t.nt) * a.KB;
-                w0 = a.sw0 + at;
-                w1 = GLU ? a.sw1 + at : nullptr;
-            }
-            const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16);
-            const int units = FP8 ? kb1 - kb0 : 1;
-            for (int i = 0; i < units; ++i, ++un) {
-                if (FP8 && i % kChunk == 0) {
-                    // the next blocks' token scales
-                    if (i) bar_sync(1, 128);
-                    const int nb = min(kChunk, units - i);
-                    for (int v = et; v < nb * BN; v += 128) {
-                        const int b = v / BN, j = v % BN;
-                        s_sx[v] = j < np ? a.sx[(size_t)(kb0 + i + b) * a.P + t.row0 + j] : 0.0f;
-                    }
-                    bar_sync(1, 128);
-                }
-                const float f0 = FP8 ? __ldg(w0 + kb0 + i) : 1.0f, f1 = FP8 && GLU ? __ldg(w1 + kb0 + i) : 1.0f;
-                const uint32_t u = un % C::kUnits;
-                wait(&acc_full[u], (un / C::kUnits) & 1);
-                tc_fence_after();
-                constexpr int kStep = BN < 32 ? 16 : 32;
-#pragma unroll
-                for (int c = 0; c < BN / kStep; ++c) {
-                    uint32_t dv[NMAT][32];
-#pragma unroll
-                    for (int m = 0; m < NMAT; ++m) {
-                        if constexpr (kStep == 16) tmem_ld16(tq + u * C::kCols + m * BN + c * 16, dv[m]);
-                        else tmem_ld32(tq + u * C::kCols + m * BN + c * 32, dv[m]);
-                    }
-                    tmem_wait_ld();
-                    if (c == BN / kStep - 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&acc_empty[u]);
-                    }
-                    if (FP8) {
-                        const float4 *sx = reinterpret_cast<const float4 *>(s_sx + (i % kChunk) * BN + c * kStep);
-#pragma unroll
-                        for (int j4 = 0; j4 < kStep / 4; ++j4) {
-                            const float4 s = sx[j4];
-                            const int j = c * kStep + 4 * j4;
-                            fma2(acc[0][j], acc[0][j + 1], dv[0][4 * j4], dv[0][4 * j4 + 1], s.x * f0, s.y * f0);
-                            fma2(acc[0][j + 2], acc[0][j + 3], dv[0][4 * j4 + 2], dv[0][4 * j4 + 3], s.z * f0,
-                                 s.w * f0);
-                            if (GLU) {
-                                constexpr int M = NMAT - 1;
-                                fma2(acc[M][j], acc[M][j + 1], dv[M][4 * j4], dv[M][4 * j4 + 1], s.x * f1, s.y * f1);
-                                fma2(acc[M][j + 2], acc[M][j + 3], dv[M][4 * j4 + 2], dv[M][4 * j4 + 3], s.z * f1,
-                                     s.w * f1);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int m = 0; m < NMAT; ++m)
-#pragma unroll
-                            for (int j = 0; j < kStep; ++j) acc[m][c * kStep + j] = __uint_as_float(dv[m][j]);
-                    }
-                }
-            }
-            if (SPLIT) {
-#pragma unroll
-                for (int m = 0; m < NMAT; ++m)
-#pragma unroll
-                    for (int j = 0; j < BN; ++j) s_part[(m * BN + j) * kLanes + row] = acc[m][j];
-            } else {
-                if (!FP8) bar_sync(1, 128);         // s_row, s_rs
-#pragma unroll
-                for (int j = 0; j < BN; ++j) {
-                    float v;
-                    if (GLU) {
-                        v = glu_value(acc[0][j], acc[NMAT - 1][j], a.act);
-                    } else {
-                        v = acc[0][j];
-                        if (a.out_f32) {
-                            const int o = s_row[j], n = t.nt * kLanes + row;
-                            if (o >= 0 && n < a.N) static_cast<float *>(a.out)[o * a.out_stride + n] = v;
-                            continue;
-                        }
-                        v = bf16r(v);
-                        if (a.row_scale) v = bf16r(v * s_rs[j]);
-                    }
-                    const uint32_t b = __float_as_uint(v) >> 16;
-                    if (GLU) {
-                        const uint32_t m = __reduce_max_sync(0xffffffffu,
-                                                             t.nt * kLanes + row < a.N ? b & 0x7FFFu : 0u);
-                        if (lane == 0) atomicMax(&s_amax[j], m);
-                    }
-                    s_out[j * kLanes + row] = (uint16_t)b;
-                }
-            }
-            if (!SPLIT) {
-                bar_sync(1, 128);
-                const int nc = (min(kLanes, a.N - t.nt * kLanes) + 15) / 16;   // 16-column pieces
-                for (int v = et; v < np * 8; v += 128) {
-                    const int j = v >> 3, c = v & 7;
-                    if (c >= nc) continue;
-                    const uint4 *p = reinterpret_cast<const uint4 *>(s_out + j * kLanes + c * 16);
-                    const uint4 lo = p[0], hi = p[1];
-                    if (GLU) {
-                        const QScale qs = qscale(s_amax[j]);
-                        const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                        uint32_t o[4];
-#pragma unroll
-                        for (int z = 0; z < 4; ++z)
-                            o[z] = cvt_e4m3x2(quotient(bf_lo(w[2 * z]), qs), quotient(bf_hi(w[2 * z]), qs)) |
-                                   (cvt_e4m3x2(quotient(bf_lo(w[2 * z + 1]), qs),
-                                               quotient(bf_hi(w[2 * z + 1]), qs)) << 16);
-                        const size_t r = (size_t)(t.row0 + j);
-                        *reinterpret_cast<uint4 *>(a.q_out + r * a.N + t.nt * kLanes + c * 16) =
-                            make_uint4(o[0], o[1], o[2], o[3]);
-                        if (c == 0) a.s_out[(size_t)t.nt * a.P + r] = qs.s;
-                    } else if (!a.out_f32) {
-                        uint4 *o = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) +
-                                                             s_row[j] * a.out_stride + t.nt * kLanes + c * 16);
-                        o[0] = lo;
-                        o[1] = hi;
-                    }
-                }
-            }
-        }
-    }
-    __syncwarp();
-    if (SPLIT) {
-        // the cluster's partial sums, added in rank order: CTA `part` takes
-        // its share of the tile's tokens
-        cluster_arrive_wait();
-        if (warp >= 2 && first < tiles) {
-            const Tile t = locate(a, s_g, first, ntiles, BN);
-            const int np = min(BN, t.end - t.row0);
-            const int row = 32 * (warp & 3) + lane, n = t.nt * kLanes + row;
-            const int j0 = BN * part / S, j1 = min(BN * (part + 1) / S, np);
-            const uint32_t pbase = smem_u32(s_part);
-            for (int j = j0; j < j1; ++j) {
-                float v[NMAT];
-#pragma unroll
-                for (int m = 0; m < NMAT; ++m) {
-                    v[m] = 0.0f;
-                    for (int c = 0; c < S; ++c) v[m] += ld_cluster(pbase + 4 * ((m * BN + j) * kLanes + row), c);
-                }
-                if (GLU) {
-                    const uint32_t b = __float_as_uint(glu_value(v[0], v[NMAT - 1], a.act)) >> 16;
-                    const uint32_t m = __reduce_max_sync(0xffffffffu, n < a.N ? b & 0x7FFFu : 0u);
-                    if (lane == 0) atomicMax(&s_amax[j], m);
-                    s_out[j * kLanes + row] = (uint16_t)b;
-                } else if (n < a.N) {
-                    const int o = s_row[j];
-                    if (a.out_f32) {
-                        static_cast<float *>(a.out)[o * a.out_stride + n] = v[0];
-                    } else {
-                        float y = bf16r(v[0]);
-                        if (a.row_scale) y = bf16r(y * s_rs[j]);
-                        static_cast<uint16_t *>(a.out)[o * a.out_stride + n] = f32_to_bf16(y);
-                    }
-                }
-            }
-            if (GLU) {
-                bar_sync(1, 128);
-                for (int j = j0; j < j1; ++j) {
-                    const QScale qs = qscale(s_amax[j]);
-                    const size_t r = (size_t)(t.row0 + j);
-                    if (n < a.N)
-                        a.q_out[r * a.N + n] =
-                            (uint8_t)cvt_e4m3x2(quotient(bf16_to_f32(s_out[j * kLanes + row]), qs), 0.0f);
-                    if (row == 0) a.s_out[(size_t)t.nt * a.P + r] = qs.s;
-                }
-            }
-        }
-        __syncwarp();
-        cluster_arrive_wait();                      // the others have read this CTA's sums
-    }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(C::kAlloc) : "memory");
-    }
-}
-
-// ------------------------------------------ many tokens: tokens as the MMA's M
-
-constexpr int kCols = 256;                     // weight rows of a tile (gate/up: 128 of each)
-constexpr int kMStages = 4;
-constexpr int kMStageBytes = kTileBytes + kCols * 128;
-constexpr size_t kMSmem = 1024 + (size_t)kMStages * kMStageBytes;
-constexpr int kMThreads = 384;                 // TMA, MMA, two idle warps, eight epilogue warps
+constexpr int kAccCols = 256;                  // accumulator columns: two halves of 128
+constexpr int kThreads = 384;                  // TMA, MMA, two idle warps, eight epilogue warps
 constexpr int kCtlRegs = 40, kEpiRegs = 232;   // setmaxnreg: 128 x 40 + 256 x 232 = 384 x 168
+constexpr int kGroup = 4, kSlots = 3;          // scale blocks of a slot of staged scales, and the slots
+constexpr int kMaxStages = 8;
+constexpr int kRingBytes = 160 * 1024;
+constexpr int kPartPitch = 257;                // floats of a row of partial sums (kSplit)
+constexpr int kPatch = 4096;                   // an epilogue warp's output staging: 32 rows of 128 bytes
+constexpr size_t kSmem = 1024 + kRingBytes + 8 * kPatch;
 
 // SwiGLU / GeGLU of two columns, every step rounded to bf16: packed bf16
 __device__ __forceinline__ uint32_t glu_pair(float g0, float g1, float u0, float u1, int act) {
@@ -604,92 +298,200 @@ __device__ __forceinline__ uint32_t glu_pair(float g0, float g1, float u0, float
     return cvt_bf16x2(bf_lo(a) * bf_lo(u), bf_hi(a) * bf_hi(u));
 }
 
-template <bool GLU, bool FP8>
-__global__ void __launch_bounds__(kMThreads, 1)
-    tok_m_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw0,
-                 const __grid_constant__ CUtensorMap tw1, const GmmArgs a) {
+// What the launcher fixes beyond GmmArgs.
+struct Plan {
+    int bm;              // token rows a CTA loads for a tile (32, 64 or 128)
+    int box;             // weight rows of one TMA copy (256, 128 or 64)
+    int stages;
+    int split;           // kSplit: CTAs of a cluster
+    int weights_first;   // the first stages' weights may be read before the kernel's predecessor has finished
+};
+
+// The 32 rows a warp's lanes hold, through its patch of shared memory, so that
+// a store instruction writes whole rows: lane `lane` puts CH 16-byte chunks of
+// its row (put), and CH lanes then write each row (flush). A thread storing its
+// own row, 16 bytes in each of 32 rows an instruction, took 12800 cycles of a
+// 128 x 256 tile; this takes 1400.
+template <int CH>
+struct RowStore {
+    uint8_t *patch;
+    int lane;
+    __device__ static int at(int row, int c) {
+        return row * (CH * 16) + 16 * (c ^ (CH == 8 ? row & 7 : (row >> 1) & 3));
+    }
+    __device__ void put(int c, uint32_t a, uint32_t b, uint32_t d, uint32_t e) const {
+        *reinterpret_cast<uint4 *>(patch + at(lane, c)) = make_uint4(a, b, d, e);
+    }
+    // row of lane l to base + row_l * pitch (bytes); row_l < 0: not stored;
+    // `valid` bytes of the row's CH * 16
+    __device__ void flush(uint8_t *base, long long pitch, int row, int valid) const {
+        __syncwarp();
+        const int c = lane % CH;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            const int rr = (32 / CH) * k + lane / CH;
+            const int o = __shfl_sync(0xffffffffu, row, rr);
+            if (o >= 0 && 16 * c < valid)
+                *reinterpret_cast<uint4 *>(base + o * pitch + 16 * c) = *reinterpret_cast<const uint4 *>(patch + at(rr, c));
+        }
+        __syncwarp();
+    }
+};
+
+template <bool GLU, bool FP8, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+    gmm_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw0,
+               const __grid_constant__ CUtensorMap tw1, const GmmArgs a, const Plan p) {
+    constexpr bool PAIR = MODE == kPair, SPLIT = MODE == kSplit;
+    constexpr int kOutCols = GLU ? 128 : 256;      // output columns of a tile
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t full[kMStages], empty[kMStages], acc_full[2], acc_empty[2];
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t s_tmem;
     __shared__ Groups s_g;
     __shared__ uint32_t s_amax[GLU ? 2 * kLanes : 1];
+    // staged products of token and weight scales: [slot][block][half, or gate / up][row]
+    __shared__ float s_scale[FP8 ? kSlots * kGroup * 2 * kLanes : 1];
+    __shared__ uint64_t sc_full[kSlots], sc_empty[kSlots];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int bm = PAIR ? kLanes : p.bm, stages = p.stages;
+    const int abytes = bm * 128, stage_bytes = abytes + (PAIR ? 128 : 256) * 128;
+    // rank in the cluster; a pair's leader (rank 0) owns the barriers its MMAs wait on
+    const int S = PAIR ? 2 : SPLIT ? p.split : 1;
+    const int rank = PAIR || SPLIT ? (int)(blockIdx.x % S) : 0;
+    const int first = blockIdx.x / S, step = gridDim.x / S;
     if (tid == 0) {
-        for (int i = 0; i < kMStages; ++i) {
+        for (int i = 0; i < stages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 8);
+            mbar_init(&acc_empty[i], PAIR ? 16 : 8);
+        }
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(&sc_full[i], 2);
+            mbar_init(&sc_empty[i], 8);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)),
-                     "r"(512)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)),
+                         "r"(512)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)),
+                         "r"(512)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        }
+    }
+    const int ntiles = (a.N + kOutCols - 1) / kOutCols;
+    const int tile_rows = PAIR ? 2 * kLanes : bm;
+    const int kb0 = SPLIT ? (int)((long long)a.KB * rank / S) : 0;
+    const int kb1 = SPLIT ? (int)((long long)a.KB * (rank + 1) / S) : a.KB;
+    Waiter wait{a.err};
+    // A stage's weights: 256 rows, in the order of the accumulator's columns;
+    // a pair's CTA loads the 128 of its rank. Gate/up: a half is 64 gate rows,
+    // then the same 64 up rows.
+    auto load_weights = [&](uint32_t dst, int kb, int wrow, uint64_t *bar) {
+        if (PAIR && GLU) {
+            tma_load_2d_pair(dst, &tw0, kb * 128, wrow + 64 * rank, bar);
+            tma_load_2d_pair(dst + 8192, &tw1, kb * 128, wrow + 64 * rank, bar);
+        } else if (PAIR) {
+            tma_load_2d_pair(dst, &tw0, kb * 128, wrow + 128 * rank, bar);
+        } else if (GLU) {
+            for (int h = 0; h < 2; ++h) {
+                tma_load_2d(dst + h * 16384, &tw0, kb * 128, wrow + 64 * h, bar);
+                tma_load_2d(dst + h * 16384 + 8192, &tw1, kb * 128, wrow + 64 * h, bar);
+            }
+        } else {
+            tma_load_2d(dst, &tw0, kb * 128, wrow, bar);
+        }
+    };
+    // A dense product's weights do not depend on the kernel before this one:
+    // the first stages' weights are on their way before its result is waited
+    // for.
+    int early = 0;
+    if (!PAIR && p.weights_first && warp == 0) {
+        if (first < ((a.P + bm - 1) / bm) * ntiles) early = min(stages, kb1 - kb0);
+        if (elect_one()) {
+            for (int s = 0; s < early; ++s) {
+                arrive_expect_tx(&full[s], stage_bytes);
+                load_weights(sbase + s * stage_bytes + abytes, kb0 + s, (first % ntiles) * kOutCols, &full[s]);
+            }
+        }
+        __syncwarp();
     }
     pdl_wait();
     pdl_trigger();
-    if (a.off && warp == 0) build_groups(a, s_g, kLanes);
+    if (a.off && warp == 0) build_groups(a, s_g, tile_rows);
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_arrive_wait();                // the peer's barriers and accumulators exist
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    constexpr int kOutCols = GLU ? 128 : kCols;    // output columns of a tile
-    const int ntiles = (a.N + kOutCols - 1) / kOutCols;
-    const int tiles = (a.off ? s_g.pre[a.E] : (a.P + kLanes - 1) / kLanes) * ntiles;
-    Waiter wait{a.err};
+    const int tiles = (a.off ? s_g.pre[a.E] : (a.P + tile_rows - 1) / tile_rows) * ntiles;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kCtlRegs));
         if (warp == 0) {
             // ---- TMA producer
             int s = 0;
-            uint32_t phase = 1;
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                const Tile t = locate(a, s_g, tile, ntiles, kLanes);
+            uint32_t phase = 1;                     // an empty stage's first wait passes
+            for (int tile = first; tile < tiles; tile += step) {
+                const Tile t = locate(a, s_g, tile, ntiles, tile_rows);
                 const int wrow = t.e * a.N + t.nt * kOutCols;
-                for (int kb = 0; kb < a.KB; ++kb) {
-                    const uint32_t st = sbase + s * kMStageBytes;
+                const int row0 = t.row0 + (PAIR ? kLanes * rank : 0);
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    const uint32_t st = sbase + s * stage_bytes;
                     wait(&empty[s], phase);
                     if (elect_one()) {
-                        arrive_expect_tx(&full[s], kMStageBytes);
-                        tma_load_2d(st, &tx, kb * 128, t.row0, &full[s]);
-                        tma_load_2d(st + kTileBytes, &tw0, kb * 128, wrow, &full[s]);
-                        if (GLU) tma_load_2d(st + 2 * kTileBytes, &tw1, kb * 128, wrow, &full[s]);
+                        if (PAIR) {
+                            // the leader's barrier counts both CTAs' bytes
+                            if (rank == 0) arrive_expect_tx(&full[s], 2 * stage_bytes);
+                            tma_load_2d_pair(st, &tx, kb * 128, row0, &full[s]);
+                            load_weights(st + abytes, kb, wrow, &full[s]);
+                        } else {
+                            if (early <= 0) {
+                                arrive_expect_tx(&full[s], stage_bytes);
+                                load_weights(st + abytes, kb, wrow, &full[s]);
+                            }
+                            tma_load_2d(st, &tx, kb * 128, row0, &full[s]);
+                        }
                     }
                     __syncwarp();
-                    if (++s == kMStages) {
+                    --early;
+                    if (++s == stages) {
                         s = 0;
                         phase ^= 1;
                     }
                 }
             }
-        } else if (warp == 1) {
-            // ---- MMA issuer: one accumulator a scale block (e4m3) or a tile (bf16)
-            constexpr uint32_t idesc = idesc_of(FP8, kCols);
+        } else if (warp == 1 && rank_issues<PAIR>(rank)) {
+            // ---- MMA issuer: the sum of one scale block (e4m3) or of a tile
+            // (bf16) at a time
+            constexpr uint32_t idesc = idesc_of(FP8, PAIR ? 256 : 128, kAccCols);
             int s = 0;
             uint32_t phase = 0, u = 0, uphase = 1;
-            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-                for (int kb = 0; kb < a.KB; ++kb) {
-                    const bool fresh = FP8 || kb == 0, last = FP8 || kb == a.KB - 1;
-                    if (fresh) wait(&acc_empty[u], uphase);
+            for (int tile = first; tile < tiles; tile += step) {
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    const bool fresh = FP8 || kb == kb0, last = FP8 || kb == kb1 - 1;
                     wait(&full[s], phase);
+                    if (fresh) wait(&acc_empty[u], uphase);
                     tc_fence_after();
-                    const uint32_t st = sbase + s * kMStageBytes, d = tmem + u * kCols;
+                    const uint32_t st = sbase + s * stage_bytes, d = tmem + u * kAccCols;
                     if (elect_one()) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
-                            mma_ss<FP8>(d, sw128_desc(st + 32 * q), sw128_desc(st + kTileBytes + 32 * q), idesc,
-                                        !fresh || q > 0);
-                        tc_commit(&empty[s]);
-                        if (last) tc_commit(&acc_full[u]);
+                            mma_ss<FP8, PAIR>(d, sw128_desc(st + 32 * q), sw128_desc(st + abytes + 32 * q), idesc,
+                                              !fresh || q > 0);
+                        commit<PAIR>(&empty[s]);
+                        if (last) commit<PAIR>(&acc_full[u]);
                     }
                     __syncwarp();
-                    if (++s == kMStages) {
+                    if (++s == stages) {
                         s = 0;
                         phase ^= 1;
                     }
@@ -700,131 +502,300 @@ __global__ void __launch_bounds__(kMThreads, 1)
                 }
             }
         }
+        else if (FP8 && warp >= 2) {
+            // ---- scales: warps 2 and 3 stage the products of the scales for
+            // the epilogue, a few blocks ahead of it. (Loaded by the epilogue
+            // itself, however far ahead, they cost it their latency in every
+            // block: 1240 cycles a block against 640.)
+            const int l = tid - 64;                 // rows l and l + 64
+            const int NB = (a.N + kScaleBlock - 1) / kScaleBlock, units = kb1 - kb0;
+            int slot = 0;
+            uint32_t phase = 1;
+            for (int tile = first; tile < tiles; tile += step) {
+                const Tile t = locate(a, s_g, tile, ntiles, tile_rows);
+                const int nb = GLU ? t.nt : 2 * t.nt;
+                const float *w0 = a.sw0 + ((size_t)t.e * NB + nb) * a.KB + kb0;
+                const float *w1 = GLU ? a.sw1 + ((size_t)t.e * NB + nb) * a.KB + kb0 : w0 + (nb + 1 < NB ? a.KB : 0);
+                const int r = t.row0 + (PAIR ? kLanes * rank : 0) + l;
+                const float *x0 = a.sx + (size_t)kb0 * a.P + min(r, a.P - 1), *x1 = x0 + min(64, a.P - 1 - min(r, a.P - 1));
+                for (int i0 = 0; i0 < units; i0 += kGroup) {
+                    float v[kGroup][4];
+#pragma unroll
+                    for (int z = 0; z < kGroup; ++z) {
+                        const int i = min(i0 + z, units - 1);
+                        v[z][0] = __ldg(x0 + (size_t)i * a.P);
+                        v[z][1] = __ldg(x1 + (size_t)i * a.P);
+                        v[z][2] = __ldg(w0 + i);
+                        v[z][3] = __ldg(w1 + i);
+                    }
+                    wait(&sc_empty[slot], phase);
+                    float *to = s_scale + slot * kGroup * 2 * kLanes + l;
+#pragma unroll
+                    for (int z = 0; z < kGroup; ++z, to += 2 * kLanes) {
+                        to[0] = v[z][0] * v[z][2];
+                        to[64] = v[z][1] * v[z][2];
+                        to[kLanes] = v[z][0] * v[z][3];
+                        to[kLanes + 64] = v[z][1] * v[z][3];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_full[slot]);
+                    if (++slot == kSlots) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (SPLIT) {
+            cluster_arrive_wait();
+            cluster_arrive_wait();
+        }
     } else {
-        // ---- epilogue: thread = one token, half of the tile's columns: 128
-        // weight rows, or (gate/up) 64 of each matrix
+        // ---- epilogue: thread = one token, one half of the tile's columns:
+        // 128 weight rows, or (gate/up) 64 of each matrix
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpiRegs));
         const int q = warp & 3, half = (warp - 4) >> 2, row = 32 * q + lane;
-        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16);
-        // its accumulator columns in four pieces of 32
-        auto piece = [&](int c) -> uint32_t { return GLU ? 64 * half + (c & 1) * 32 + (c >> 1) * 128 : 128 * half + 32 * c; };
-        const int NB = (a.N + kScaleBlock - 1) / kScaleBlock;
-        uint32_t un = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            const Tile t = locate(a, s_g, tile, ntiles, kLanes);
-            const int r = t.row0 + row;
-            const bool live = r < t.end;
-            const int n0 = t.nt * kOutCols + piece(0);   // its first output column
-            float acc[128];
-            const float *w0 = nullptr, *w1 = nullptr;
+        const bool busy = 32 * q < bm;              // lanes that hold token rows at all
+        uint8_t *const patch = smem_raw + (sbase - smem_u32(smem_raw)) + kRingBytes + (warp - 4) * kPatch;
+        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + half * 128;
+        uint32_t un = 0, sphase = 0;
+        int slot = 0;
+        for (int tile = first; tile < tiles; tile += step) {
+            const Tile t = locate(a, s_g, tile, ntiles, tile_rows);
+            const int r = t.row0 + (PAIR ? kLanes * rank : 0) + row;
+            const bool live = row < bm && r < t.end;
+            const int n0 = t.nt * kOutCols + half * (kOutCols / 2);   // its first output column
+            uint64_t acc[64];                       // 128 float32 sums
             if (FP8) {
 #pragma unroll
-                for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-                const size_t at = ((size_t)t.e * NB + min(n0 / kScaleBlock, NB - 1)) * a.KB;
-                w0 = a.sw0 + at;
-                w1 = GLU ? a.sw1 + at : w0;
+                for (int j = 0; j < 64; ++j) acc[j] = 0;
             }
-            const int units = FP8 ? a.KB : 1;
-            float sx = FP8 && live ? __ldg(a.sx + r) : 0.0f;
-            float f0 = FP8 ? __ldg(w0) : 1.0f, f1 = FP8 && GLU ? __ldg(w1) : 1.0f;
-            for (int i = 0; i < units; ++i, ++un) {
-                const float s0 = sx * f0, s1 = GLU ? sx * f1 : s0;
-                if (FP8 && i + 1 < units) {            // the next block's scales
-                    if (live) sx = __ldg(a.sx + (size_t)(i + 1) * a.P + r);
-                    f0 = __ldg(w0 + i + 1);
-                    if (GLU) f1 = __ldg(w1 + i + 1);
-                }
-                const uint32_t u = un & 1, td = tq + u * kCols;
-                wait(&acc_full[u], (un >> 1) & 1);
-                tc_fence_after();
-                uint32_t dv[2][32];
-                auto add = [&](int c) {
-                    const float s = c >= 2 ? s1 : s0;
+            const int units = FP8 ? kb1 - kb0 : 1;
+            for (int i0 = 0; i0 < units; i0 += kGroup) {
+                if (FP8) wait(&sc_full[slot], sphase);
+                const float *sc = s_scale + slot * kGroup * 2 * kLanes + row;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        if (FP8) {
-                            fma2(acc[32 * c + j], acc[32 * c + j + 1], dv[c & 1][j], dv[c & 1][j + 1], s, s);
-                        } else {
-                            acc[32 * c + j] = __uint_as_float(dv[c & 1][j]);
-                            acc[32 * c + j + 1] = __uint_as_float(dv[c & 1][j + 1]);
+                for (int z = 0; z < kGroup; ++z) {
+                    if (i0 + z >= units) break;
+                    uint64_t s0 = 0, s1 = 0;
+                    if (FP8) {
+                        const uint32_t b = __float_as_uint(sc[(2 * z + (GLU ? 0 : half)) * kLanes]);
+                        s0 = s1 = pack2(b, b);
+                        if (GLU) {
+                            const uint32_t c = __float_as_uint(sc[(2 * z + 1) * kLanes]);
+                            s1 = pack2(c, c);
                         }
                     }
-                };
-                tmem_ld32(td + piece(0), dv[0]);
-                tmem_ld32(td + piece(1), dv[1]);
-                tmem_wait_ld();
-                add(0);
-                tmem_ld32(td + piece(2), dv[0]);
-                add(1);
-                tmem_ld32(td + piece(3), dv[1]);
-                tmem_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[u]);
-                add(2);
-                add(3);
+                    const uint32_t u = un & 1, td = tq + u * kAccCols;
+                    wait(&acc_full[u], (un >> 1) & 1);
+                    ++un;
+                    tc_fence_after();
+                    uint32_t dv[2][32];
+                    auto add = [&](int c) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const uint64_t v = pack2(dv[c & 1][2 * j], dv[c & 1][2 * j + 1]);
+                            if (FP8) fma2(acc[16 * c + j], v, c < 2 ? s0 : s1);
+                            else acc[16 * c + j] = v;
+                        }
+                    };
+                    if (busy) {
+                        tmem_ld32(td, dv[0]);
+                        tmem_ld32(td + 32, dv[1]);
+                        tmem_wait_ld();
+                        add(0);
+                        tmem_ld32(td + 64, dv[0]);
+                        add(1);
+                        tmem_ld32(td + 96, dv[1]);
+                        tmem_wait_ld();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive<PAIR>(&acc_empty[u]);
+                    if (busy) {
+                        add(2);
+                        add(3);
+                    }
+                }
+                if (FP8) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_empty[slot]);
+                    if (++slot == kSlots) {
+                        slot = 0;
+                        sphase ^= 1;
+                    }
+                }
             }
-            if (GLU) {
+            if (SPLIT) {
+                // the ring is idle: this CTA's sums, [row][column], rows at
+                // a pitch of 257 so that lanes (rows) meet no bank twice and
+                // the others read a row's columns in whole lines
+                float *part = reinterpret_cast<float *>(smem_raw + (sbase - smem_u32(smem_raw)));
+                if (row < bm) {
+                    float *to = part + row * kPartPitch + half * 128;
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) {
+                        to[2 * j] = lo2(acc[j]);
+                        to[2 * j + 1] = hi2(acc[j]);
+                    }
+                }
+            } else if (GLU) {
                 // 64 activations of the token's group of 128; the largest of
                 // all 128 with the other half's warp
                 uint32_t m = 0, v[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
-                    v[j] = glu_pair(acc[2 * j], acc[2 * j + 1], acc[64 + 2 * j], acc[65 + 2 * j], a.act);
+                    v[j] = glu_pair(lo2(acc[j]), hi2(acc[j]), lo2(acc[32 + j]), hi2(acc[32 + j]), a.act);
                     if (n0 + 2 * j < a.N) m = __vmaxu2(m, v[j] & 0x7FFF7FFFu);
                 }
                 m = max(m & 0xFFFFu, m >> 16);
                 s_amax[half * kLanes + row] = m;
                 bar_sync(1, 256);
                 m = max(m, s_amax[(half ^ 1) * kLanes + row]);
-                bar_sync(1, 256);                      // read before the next tile's
+                bar_sync(1, 256);                   // read before the next tile's
                 const QScale qs = qscale(m);
-                if (live) {
-                    uint8_t *o = a.q_out + (size_t)r * a.N + n0;
+                const RowStore<4> rows{patch, lane};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t w[4];
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const uint32_t x0 = v[8 * c + 2 * z], x1 = v[8 * c + 2 * z + 1];
-                            w[z] = cvt_e4m3x2(quotient(bf_lo(x0), qs), quotient(bf_hi(x0), qs)) |
-                                   (cvt_e4m3x2(quotient(bf_lo(x1), qs), quotient(bf_hi(x1), qs)) << 16);
-                        }
-                        if (n0 + 16 * c < a.N) reinterpret_cast<uint4 *>(o)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int z = 0; z < 4; ++z) {
+                        const uint32_t x0 = v[8 * c + 2 * z], x1 = v[8 * c + 2 * z + 1];
+                        w[z] = cvt_e4m3x2(quotient(bf_lo(x0), qs), quotient(bf_hi(x0), qs)) |
+                               (cvt_e4m3x2(quotient(bf_lo(x1), qs), quotient(bf_hi(x1), qs)) << 16);
                     }
-                    if (half == 0) a.s_out[(size_t)t.nt * a.P + r] = qs.s;
+                    rows.put(c, w[0], w[1], w[2], w[3]);
                 }
-            } else if (live) {
-                const int o = a.map ? a.map[r] : r;
+                rows.flush(a.q_out + n0, a.N, live ? r : -1, a.N - n0);
+                if (half == 0 && live) a.s_out[(size_t)t.nt * a.P + r] = qs.s;
+            } else {
+                const int o = live ? (a.map ? a.map[r] : r) : -1;
+                const RowStore<8> rows{patch, lane};
                 if (a.out_f32) {
-                    float *p = static_cast<float *>(a.out) + o * a.out_stride + n0;
+                    uint8_t *y = reinterpret_cast<uint8_t *>(static_cast<float *>(a.out) + n0);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (n0 + 4 * c < a.N)
-                            reinterpret_cast<float4 *>(p)[c] =
-                                make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
-                } else {
-                    const float rs = a.row_scale ? a.row_scale[o] : 1.0f;
-                    uint16_t *p = static_cast<uint16_t *>(a.out) + o * a.out_stride + n0;
+                    for (int h = 0; h < 4; ++h) {
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            w[z] = cvt_bf16x2(acc[8 * c + 2 * z], acc[8 * c + 2 * z + 1]);
-                            if (a.row_scale) w[z] = cvt_bf16x2(bf_lo(w[z]) * rs, bf_hi(w[z]) * rs);
+                        for (int c = 0; c < 8; ++c) {
+                            const uint64_t x0 = acc[16 * h + 2 * c], x1 = acc[16 * h + 2 * c + 1];
+                            rows.put(c, (uint32_t)x0, (uint32_t)(x0 >> 32), (uint32_t)x1, (uint32_t)(x1 >> 32));
                         }
-                        if (n0 + 8 * c < a.N) reinterpret_cast<uint4 *>(p)[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                        rows.flush(y + 128 * h, 4 * a.out_stride, o, 4 * (a.N - n0) - 128 * h);
+                    }
+                } else {
+                    const float rs = a.row_scale && o >= 0 ? a.row_scale[o] : 1.0f;
+                    uint8_t *y = reinterpret_cast<uint8_t *>(static_cast<uint16_t *>(a.out) + n0);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) {
+                                const uint64_t x = acc[32 * h + 4 * c + z];
+                                w[z] = cvt_bf16x2(lo2(x), hi2(x));
+                                if (a.row_scale) w[z] = cvt_bf16x2(bf_lo(w[z]) * rs, bf_hi(w[z]) * rs);
+                            }
+                            rows.put(c, w[0], w[1], w[2], w[3]);
+                        }
+                        rows.flush(y + 128 * h, 2 * a.out_stride, o, 2 * (a.N - n0) - 128 * h);
                     }
                 }
             }
         }
+        __syncwarp();
+        if (SPLIT) {
+            // Each CTA adds up and stores its share of the tile: a warp takes 32
+            // columns of a row, or (gate/up) a row's 128 activations.
+            cluster_arrive_wait();
+            if (first < tiles) {
+                const Tile t = locate(a, s_g, first, ntiles, tile_rows);
+                const int np = min(bm, t.end - t.row0);
+                uint32_t peer[8];
+    #pragma unroll
+                for (int c = 0; c < 8; ++c) peer[c] = map_cluster(sbase, min(c, S - 1));
+                // the cluster's sums of N (row, column)s, every load in flight
+                // before the first is used
+                auto sums = [&](auto &v, const auto &at) {
+                    constexpr int N = sizeof(v) / sizeof(float);
+                    float x[N][8];
+    #pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (c < S)
+    #pragma unroll
+                            for (int n = 0; n < N; ++n) x[n][c] = ld_cluster(peer[c] + 4 * at(n));
+    #pragma unroll
+                    for (int n = 0; n < N; ++n) v[n] = 0.0f;
+    #pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (c < S)
+    #pragma unroll
+                            for (int n = 0; n < N; ++n) v[n] += x[n][c];
+                };
+                if (GLU) {
+                    for (int u = (warp - 4) * S + rank; u < np; u += 8 * S) {
+                        float g[8], v[4];            // gate and up of this lane's four columns
+                        uint32_t m = 0;
+                        sums(g, [&](int n) {
+                            const int c = lane + 32 * (n & 3);
+                            return u * kPartPitch + (c >> 6) * 128 + (c & 63) + 64 * (n >> 2);
+                        });
+    #pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t y = glu_pair(g[i], 0.0f, g[4 + i], 0.0f, a.act);
+                            v[i] = bf_lo(y);
+                            if (t.nt * 128 + lane + 32 * i < a.N) m = max(m, y & 0x7FFFu);
+                        }
+                        const QScale qs = qscale(__reduce_max_sync(0xffffffffu, m));
+                        const size_t r = (size_t)(t.row0 + u);
+    #pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int n = t.nt * 128 + lane + 32 * i;
+                            if (n < a.N) a.q_out[r * a.N + n] = (uint8_t)cvt_e4m3x2(quotient(v[i], qs), 0.0f);
+                        }
+                        if (lane == 0) a.s_out[(size_t)t.nt * a.P + r] = qs.s;
+                    }
+                } else {
+                    // 32 columns of a row a warp and step, four steps at a time
+                    constexpr int kSteps = 4;
+                    const int step8 = 8 * S, total = 8 * np;
+                    for (int u0 = (warp - 4) * S + rank; u0 < total; u0 += kSteps * step8) {
+                        float v[kSteps];
+                        sums(v, [&](int n) {
+                            const int u = min(u0 + n * step8, total - 1);
+                            return (u >> 3) * kPartPitch + (u & 7) * 32 + lane;
+                        });
+    #pragma unroll
+                        for (int k = 0; k < kSteps; ++k) {
+                            const int u = u0 + k * step8, n = t.nt * 256 + (u & 7) * 32 + lane;
+                            if (u >= total || n >= a.N) continue;
+                            const int r = t.row0 + (u >> 3), o = a.map ? a.map[r] : r;
+                            if (a.out_f32) {
+                                static_cast<float *>(a.out)[o * a.out_stride + n] = v[k];
+                            } else {
+                                float y = bf16r(v[k]);
+                                if (a.row_scale) y = bf16r(y * a.row_scale[o]);
+                                static_cast<uint16_t *>(a.out)[o * a.out_stride + n] = f32_to_bf16(y);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            cluster_arrive_wait();                      // the others have read this CTA's sums
+        }
     }
     tc_fence_before();
     __syncthreads();
+    // neither CTA of a pair leaves while the other may signal its barriers
+    if (PAIR) cluster_arrive_wait();
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+        if (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
     }
 }
 
@@ -837,16 +808,16 @@ static vqmoe_status check_registers(const void *fn) {
     static std::mutex mu;
     static std::map<std::pair<const void *, int>, int> regs;
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("tok_m_kernel");
+    if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("gmm_kernel");
     std::lock_guard<std::mutex> lock(mu);
     int &n = regs[{fn, dev}];
     if (!n) {
         cudaFuncAttributes at{};
-        if (cudaFuncGetAttributes(&at, fn) != cudaSuccess) return check_launch("tok_m_kernel");
+        if (cudaFuncGetAttributes(&at, fn) != cudaSuccess) return check_launch("gmm_kernel");
         n = at.numRegs;
     }
-    if (n * kMThreads < 128 * kCtlRegs + 256 * kEpiRegs)
-        return set_error(VQMOE_LAUNCH_FAILED, "tok_m_kernel: built with %d registers a thread", n);
+    if (n * kThreads < 128 * kCtlRegs + 256 * kEpiRegs)
+        return set_error(VQMOE_LAUNCH_FAILED, "gmm_kernel: built with %d registers a thread", n);
     return VQMOE_OK;
 }
 
@@ -856,18 +827,67 @@ static bool byte_map(CUtensorMap *m, const void *base, size_t rows, size_t row_b
     return encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, dims, pitch, box) == CUDA_SUCCESS;
 }
 
-struct Maps {
-    CUtensorMap x, w0, w1;
-};
+template <int MODE>
+static const void *kernel_of(bool glu, bool fp8) {
+    return glu   ? reinterpret_cast<const void *>(&gmm_kernel<true, true, MODE>)
+           : fp8 ? reinterpret_cast<const void *>(&gmm_kernel<false, true, MODE>)
+                 : reinterpret_cast<const void *>(&gmm_kernel<false, false, MODE>);
+}
 
-static vqmoe_status launch_with(const void *fn, const char *what, Maps &m, const GmmArgs &a, int grid, int threads,
-                                size_t smem, int cluster, const int *weights_first, cudaStream_t stream) {
-    vqmoe_status s = ensure_dynamic_smem(fn, smem, what);
-    if (s != VQMOE_OK) return s;
+}  // namespace gm
+
+vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const void *w1, size_t row_bytes, bool fp8,
+                        const GmmArgs &a, cudaStream_t stream, bool pdl_weights) {
+    using namespace gm;
+    const bool glu = w1 != nullptr;
+    if (a.P <= 0) return VQMOE_OK;
+    if (a.E <= 0 || a.E > kMaxGroups || (!a.off && a.E != 1))
+        return set_error(VQMOE_BAD_SHAPE, "grouped product: %d groups (1..%d)", a.E, kMaxGroups);
+    if ((long long)a.E * a.N > 0x7FFFFFFFLL - 256 || (long long)a.KB * 128 > 0x7FFFFFFFLL)
+        return set_error(VQMOE_BAD_SHAPE, "grouped product: %d groups of %d rows", a.E, a.N);
+    const int sms = sm_count();
+    // groups that can have rows, their mean rows, and (a bound on) the tiles of `rows` token rows
+    const int groups = std::min(a.E, a.P), mean = (a.P + groups - 1) / groups;
+    const long long ntiles = (a.N + (glu ? 127 : 255)) / (glu ? 128 : 256);
+    auto tiles_of = [&](int rows) {
+        return ntiles * (a.off ? std::min<long long>(a.P, a.P / rows + groups) : (a.P + rows - 1) / rows);
+    };
+    Plan p{};
+    p.bm = mean <= 24 ? 32 : mean <= 48 ? 64 : 128;
+    p.split = 1;
+    const char *env = getenv("GMM_MODE");
+    int mode = mean > 128 ? kPair : kSingle;
+    if (env) mode = atoi(env);
+    if (const char *b = getenv("GMM_BM")) p.bm = atoi(b);
+    if (mode != kPair) {
+        while (p.split < 8 && tiles_of(p.bm) * p.split * 2 <= sms && p.split * 4 <= a.KB) p.split *= 2;
+        mode = p.split > 1 ? kSplit : kSingle;
+    } else {
+        p.bm = kLanes;
+    }
+    const int stage = p.bm * 128 + (mode == kPair ? 128 : 256) * 128;
+    p.stages = std::min(kMaxStages, kRingBytes / stage);
+    p.box = glu ? 64 : mode == kPair ? 128 : 256;
+    p.weights_first = pdl_weights && !a.off && mode != kPair;
+    const int cluster = mode == kPair ? 2 : p.split;
+    const long long tiles = std::min<long long>(tiles_of(mode == kPair ? 256 : p.bm), 1 << 20);
+    const int grid = mode == kSplit ? (int)tiles * p.split
+                     : mode == kPair ? 2 * (int)std::min<long long>(tiles, sms / 2)
+                                     : (int)std::min<long long>(tiles, sms);
+    CUtensorMap mx, m0, m1;
+    const size_t wrows = (size_t)a.E * a.N;
+    if (!byte_map(&mx, x, a.P, row_bytes, x_pitch, p.bm) || !byte_map(&m0, w0, wrows, row_bytes, row_bytes, p.box) ||
+        !byte_map(&m1, glu ? w1 : w0, wrows, row_bytes, row_bytes, p.box))
+        return set_error(VQMOE_LAUNCH_FAILED, "grouped product: tensor map");
+    const void *fn = mode == kPair    ? kernel_of<kPair>(glu, fp8)
+                     : mode == kSplit ? kernel_of<kSplit>(glu, fp8)
+                                      : kernel_of<kSingle>(glu, fp8);
+    vqmoe_status s = check_registers(fn);
+    if (s != VQMOE_OK || (s = ensure_dynamic_smem(fn, kSmem, "gmm_kernel")) != VQMOE_OK) return s;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -877,92 +897,9 @@ static vqmoe_status launch_with(const void *fn, const char *what, Maps &m, const
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    int wf = weights_first ? *weights_first : 0;
-    void *params[5] = {&m.x, &m.w0, &m.w1, const_cast<GmmArgs *>(&a), &wf};
-    if (cudaLaunchKernelExC(&cfg, fn, params) != cudaSuccess) return check_launch(what);
+    void *params[5] = {&mx, &m0, &m1, const_cast<GmmArgs *>(&a), &p};
+    if (cudaLaunchKernelExC(&cfg, fn, params) != cudaSuccess) return check_launch("gmm_kernel");
     return VQMOE_OK;
-}
-
-template <int BN, int NMAT, bool FP8, bool SPLIT>
-static vqmoe_status launch_n(Maps &m, const GmmArgs &a, int tiles, int wf, cudaStream_t stream) {
-    using C = NCfg<BN, NMAT, FP8, SPLIT>;
-    const int grid = SPLIT ? tiles * a.split : std::min(tiles, sm_count());
-    return launch_with(reinterpret_cast<const void *>(&tok_n_kernel<BN, NMAT, FP8, SPLIT>), "tok_n_kernel", m, a, grid,
-                       kNThreads, C::kSmem, SPLIT ? a.split : 1, &wf, stream);
-}
-
-template <int BN, int NMAT, bool FP8>
-static vqmoe_status launch_n2(Maps &m, const GmmArgs &a, int tiles, int wf, cudaStream_t stream) {
-    return a.split > 1 ? launch_n<BN, NMAT, FP8, true>(m, a, tiles, wf, stream)
-                       : launch_n<BN, NMAT, FP8, false>(m, a, tiles, wf, stream);
-}
-
-}  // namespace gm
-
-vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const void *w1, size_t row_bytes, bool fp8,
-                        GmmArgs a, cudaStream_t stream, bool pdl_weights) {
-    using namespace gm;
-    const bool glu = w1 != nullptr;
-    if (a.P <= 0) return VQMOE_OK;
-    if (a.E <= 0 || a.E > kMaxGroups || (!a.off && a.E != 1))
-        return set_error(VQMOE_BAD_SHAPE, "grouped product: %d groups (1..%d)", a.E, kMaxGroups);
-    if ((long long)a.E * a.N > 0x7FFFFFFFLL - 256 || (long long)a.KB * 128 > 0x7FFFFFFFLL)
-        return set_error(VQMOE_BAD_SHAPE, "grouped product: %d groups of %d rows", a.E, a.N);
-    // groups that can have rows, and their mean rows
-    const int groups = std::min(a.E, a.P), mean = (a.P + groups - 1) / groups;
-    const int bn_max = glu ? 64 : 128;
-    const char *env = getenv("GMM_M"); const int thr = env ? atoi(env) : bn_max;
-    Maps m;
-    const size_t wrows = (size_t)a.E * a.N;
-    if (mean > thr) {
-        if (!byte_map(&m.x, x, a.P, row_bytes, x_pitch, kLanes) ||
-            !byte_map(&m.w0, w0, wrows, row_bytes, row_bytes, glu ? 128 : kCols) ||
-            !byte_map(&m.w1, glu ? w1 : w0, wrows, row_bytes, row_bytes, 128))
-            return set_error(VQMOE_LAUNCH_FAILED, "grouped product: tensor map");
-        const int out_cols = glu ? 128 : kCols;
-        const long long tiles = ((long long)a.P / kLanes + groups) * ((a.N + out_cols - 1) / out_cols);
-        const int grid = (int)std::min<long long>(tiles, sm_count());
-        a.split = 1;
-        const void *fn = glu   ? reinterpret_cast<const void *>(&tok_m_kernel<true, true>)
-                         : fp8 ? reinterpret_cast<const void *>(&tok_m_kernel<false, true>)
-                               : reinterpret_cast<const void *>(&tok_m_kernel<false, false>);
-        const vqmoe_status s = check_registers(fn);
-        if (s != VQMOE_OK) return s;
-        return launch_with(fn, "tok_m_kernel", m, a, grid, kMThreads, kMSmem, 1, nullptr, stream);
-    }
-    int bn = 16;
-    while (bn < mean && bn < bn_max) bn *= 2;
-    if (!byte_map(&m.x, x, a.P, row_bytes, x_pitch, bn) || !byte_map(&m.w0, w0, wrows, row_bytes, row_bytes, kLanes) ||
-        !byte_map(&m.w1, glu ? w1 : w0, wrows, row_bytes, row_bytes, kLanes))
-        return set_error(VQMOE_LAUNCH_FAILED, "grouped product: tensor map");
-    const long long tok_tiles = a.off ? std::min<long long>(a.P, (long long)a.P / bn + groups) : (a.P + bn - 1) / bn;
-    const long long ntiles = (a.N + kLanes - 1) / kLanes;
-    const int tiles = (int)std::min<long long>(tok_tiles * ntiles, 1 << 20);
-    // few tiles: clusters share a tile's blocks, two blocks a CTA at least
-    a.split = 1;
-    while (a.split < 8 && (long long)tiles * a.split * 2 <= sm_count() && a.split * 4 <= a.KB) a.split *= 2;
-    const int wf = pdl_weights && !a.off;
-    if (glu) {
-        switch (bn) {
-            case 16: return launch_n2<16, 2, true>(m, a, tiles, wf, stream);
-            case 32: return launch_n2<32, 2, true>(m, a, tiles, wf, stream);
-            default: return launch_n2<64, 2, true>(m, a, tiles, wf, stream);
-        }
-    }
-    if (fp8) {
-        switch (bn) {
-            case 16: return launch_n2<16, 1, true>(m, a, tiles, wf, stream);
-            case 32: return launch_n2<32, 1, true>(m, a, tiles, wf, stream);
-            case 64: return launch_n2<64, 1, true>(m, a, tiles, wf, stream);
-            default: return launch_n2<128, 1, true>(m, a, tiles, wf, stream);
-        }
-    }
-    switch (bn) {
-        case 16: return launch_n2<16, 1, false>(m, a, tiles, wf, stream);
-        case 32: return launch_n2<32, 1, false>(m, a, tiles, wf, stream);
-        case 64: return launch_n2<64, 1, false>(m, a, tiles, wf, stream);
-        default: return launch_n2<128, 1, false>(m, a, tiles, wf, stream);
-    }
 }
 
 // -------------------------------------------------------------- quantizer

@@ -26,7 +26,6 @@ struct GmmArgs {
     float *s_out;                     // ... and their scales, block-major [ceil(N / 128)][P]
     int act;                          // gate/up: VQMOE_ACT_*
     uint32_t *err;                    // word raised when a bounded wait ran out, or null
-    int split;                        // CTAs that share a tile's inputs (a cluster), set by the launcher
 };
 
 // x: rows of `row_bytes` bytes at a pitch of x_pitch bytes; w0 (and w1, the
@@ -34,7 +33,7 @@ struct GmmArgs {
 // pdl_weights: the weights may be read before the kernel's predecessor on the
 // stream has finished (nothing queued may still write them).
 vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const void *w1, size_t row_bytes, bool fp8,
-                        GmmArgs a, cudaStream_t stream, bool pdl_weights = false);
+                        const GmmArgs &a, cudaStream_t stream, bool pdl_weights = false);
 
 // bf16 rows -> e4m3 rows [..][cols] and float32 scales, element (row, g) at
 // s[row * s_row + g * s_group]. With `order` the rows of x (one for each of
