@@ -317,6 +317,10 @@ static vqmoe_status clear_status(uint32_t *status, cudaStream_t st) {
 // Tokens per launch sequence; a larger T runs as independent token chunks
 // (bounds the workspace).
 constexpr int kMaxTokensPerLaunch = 2048;
+// ... of a SwitchGLU with e4m3 experts: their tiles hold up to 256 rows of one
+// expert, which a larger launch fills better
+constexpr int kMaxTokensFp8 = 8192;
+static int launch_tokens(const vqmoe_linear *w) { return is_fp8(w->format) ? kMaxTokensFp8 : kMaxTokensPerLaunch; }
 
 // the gate linear of a SwitchGLU names its activation
 static vqmoe_status check_glu_activation(const vqmoe_linear *gate) {
@@ -588,6 +592,14 @@ static vqmoe_status run_block(const vqmoe_block *b, const uint16_t *x, int T,
     return mark(ev, n_ev, 4, st);
 }
 
+// The routing sort of given expert ids, for the kernels of `w`'s format.
+static vqmoe_status route_pairs(const vqmoe_linear *w, const int32_t *inds, int P, int E, const RouteWs &rt,
+                                cudaStream_t st) {
+    if (is_fp8(w->format) && P >= kRouteWide)
+        return launch_route_wide(inds, P, E, rt.cnt, rt.off, rt.list, rt.active, rt.rank, st);
+    return launch_route(inds, P, E, rt.cnt, rt.off, rt.list, rt.active, rt.rank, rt.zero, rt.zero_words, st);
+}
+
 // Workspace of vqmoe_switch_glu / vqmoe_switch_linear at T tokens.
 struct GluWs {
     uint32_t *status;    // kStatusBytes at offset 0: [0] routed experts
@@ -674,14 +686,14 @@ size_t vqmoe_router_workspace_size(int32_t tokens, int32_t num_experts) {
 size_t vqmoe_switch_glu_workspace_size(const vqmoe_linear *gate, const vqmoe_linear *down,
                                        int32_t tokens, int32_t top_k) {
     if (!gate || !down || tokens <= 0 || top_k <= 0) return 0;
-    const int T = std::min<int>(tokens, kMaxTokensPerLaunch);
+    const int T = std::min<int>(tokens, launch_tokens(gate));
     return carve_glu(nullptr, gate, down, T, top_k, T).bytes;
 }
 
 size_t vqmoe_switch_linear_workspace_size(const vqmoe_linear *w, int32_t tokens, int32_t top_k,
                                           int32_t x_per_pair) {
     if (!w || tokens <= 0 || top_k <= 0) return 0;
-    const int T = std::min<int>(tokens, kMaxTokensPerLaunch);
+    const int T = std::min<int>(tokens, launch_tokens(w));
     return carve_glu(nullptr, w, nullptr, T, top_k, x_per_pair ? T * top_k : T).bytes;
 }
 
@@ -855,7 +867,7 @@ vqmoe_status vqmoe_switch_glu(const vqmoe_linear *gate, const vqmoe_linear *up,
     if (E > 1024) return set_error(VQMOE_BAD_SHAPE, "switch_glu: %d experts (<= 1024)", E);
     if (!aligned_ptr(x) || !aligned_ptr(y) || !indices || !aligned_ptr(workspace))
         return set_error(VQMOE_BAD_POINTER, "x / indices / y / workspace");
-    const int chunk = std::min<int>(tokens, kMaxTokensPerLaunch);
+    const int chunk = std::min<int>(tokens, launch_tokens(gate));
     GluWs w = carve_glu(workspace, gate, down, chunk, top_k, chunk);
     if (workspace_bytes < w.bytes)
         return set_error(VQMOE_WORKSPACE_TOO_SMALL, "workspace %zu < %zu bytes", workspace_bytes, w.bytes);
@@ -868,9 +880,7 @@ vqmoe_status vqmoe_switch_glu(const vqmoe_linear *gate, const vqmoe_linear *up,
         const uint16_t *xt = static_cast<const uint16_t *>(x) + (size_t)t0 * H;
         const RouteWs &rt = w.rt;
         if (vq_in && (s = launch_to_f16(xt, w.x16, (size_t)T * H, st)) != VQMOE_OK) return s;
-        if ((s = launch_route(ind, P, E, rt.cnt, rt.off, rt.list, rt.active, rt.rank, rt.zero,
-                              rt.zero_words, st)) != VQMOE_OK)
-            return s;
+        if ((s = route_pairs(gate, ind, P, E, rt, st)) != VQMOE_OK) return s;
         RoutedIO r1 = routed_io(rt, E, top_k, P, vq_in ? (const void *)w.x16 : (const void *)xt, 0,
                                 w.act, vq_dn, nullptr);
         r1.xs = w.xs;
@@ -894,7 +904,7 @@ static size_t moe_experts_ybuf_offset(const GluWs &w) { return align_up(w.bytes,
 size_t vqmoe_moe_experts_workspace_size(const vqmoe_linear *gate, const vqmoe_linear *down, int32_t tokens,
                                         int32_t top_k) {
     if (!gate || !down || tokens <= 0 || top_k <= 0) return 0;
-    const int T = std::min<int>(tokens, kMaxTokensPerLaunch);
+    const int T = std::min<int>(tokens, launch_tokens(gate));
     const GluWs w = carve_glu(nullptr, gate, down, T, top_k, T);
     return align_up(moe_experts_ybuf_offset(w) + (size_t)T * top_k * gate->in_features * sizeof(uint16_t), 256);
 }
@@ -917,7 +927,7 @@ vqmoe_status vqmoe_moe_experts(const vqmoe_linear *gate, const vqmoe_linear *up,
     if (E > 1024) return set_error(VQMOE_BAD_SHAPE, "moe_experts: %d experts (<= 1024)", E);
     if (!aligned_ptr(x) || !aligned_ptr(out) || !indices || !scores || !aligned_ptr(workspace))
         return set_error(VQMOE_BAD_POINTER, "x / indices / scores / out / workspace");
-    const int chunk = std::min<int>(tokens, kMaxTokensPerLaunch);
+    const int chunk = std::min<int>(tokens, launch_tokens(gate));
     GluWs w = carve_glu(workspace, gate, down, chunk, top_k, chunk);
     const size_t need = vqmoe_moe_experts_workspace_size(gate, down, tokens, top_k);
     if (workspace_bytes < need)
@@ -932,9 +942,7 @@ vqmoe_status vqmoe_moe_experts(const vqmoe_linear *gate, const vqmoe_linear *up,
         const uint16_t *xt = static_cast<const uint16_t *>(x) + (size_t)t0 * H;
         const RouteWs &rt = w.rt;
         if (vq_in && (s = launch_to_f16(xt, w.x16, (size_t)T * H, st)) != VQMOE_OK) return s;
-        if ((s = launch_route(ind, P, E, rt.cnt, rt.off, rt.list, rt.active, rt.rank, rt.zero,
-                              rt.zero_words, st)) != VQMOE_OK)
-            return s;
+        if ((s = route_pairs(gate, ind, P, E, rt, st)) != VQMOE_OK) return s;
         RoutedIO r1 = routed_io(rt, E, top_k, P, vq_in ? (const void *)w.x16 : (const void *)xt, 0,
                                 w.act, vq_dn, nullptr);
         r1.xs = w.xs;
@@ -961,7 +969,7 @@ vqmoe_status vqmoe_switch_linear(const vqmoe_linear *w, const void *x, int32_t x
     if (w->num_experts > 1024) return set_error(VQMOE_BAD_SHAPE, "switch_linear: %d experts (<= 1024)", w->num_experts);
     if (!aligned_ptr(x) || !aligned_ptr(y) || !indices || !aligned_ptr(workspace))
         return set_error(VQMOE_BAD_POINTER, "x / indices / y / workspace");
-    const int chunk = std::min<int>(tokens, kMaxTokensPerLaunch);
+    const int chunk = std::min<int>(tokens, launch_tokens(w));
     const int rows_x = x_per_pair ? chunk * top_k : chunk;
     GluWs ws = carve_glu(workspace, w, nullptr, chunk, top_k, rows_x);
     if (workspace_bytes < ws.bytes)
@@ -977,9 +985,7 @@ vqmoe_status vqmoe_switch_linear(const vqmoe_linear *w, const void *x, int32_t x
         const uint16_t *xt = static_cast<const uint16_t *>(x) + xrow0 * IN;
         const RouteWs &rt = ws.rt;
         if (vq && (s = launch_to_f16(xt, ws.x16, nrows * IN, st)) != VQMOE_OK) return s;
-        if ((s = launch_route(indices + (size_t)t0 * top_k, P, E, rt.cnt, rt.off, rt.list, rt.active,
-                              rt.rank, rt.zero, rt.zero_words, st)) != VQMOE_OK)
-            return s;
+        if ((s = route_pairs(w, indices + (size_t)t0 * top_k, P, E, rt, st)) != VQMOE_OK) return s;
         RoutedIO r = routed_io(rt, E, top_k, P, vq ? (const void *)ws.x16 : (const void *)xt,
                                x_per_pair, static_cast<uint16_t *>(y) + (size_t)t0 * top_k * w->out_features,
                                0, nullptr);

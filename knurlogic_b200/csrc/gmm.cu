@@ -32,7 +32,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <cstdlib>
 #include <map>
 #include <mutex>
 
@@ -49,24 +48,31 @@ using namespace tc;
 
 constexpr int kLanes = 128;                    // rows of an accumulator (MMA M)
 
+// Whether a barrier's phase of that parity is over, without waiting
+__device__ __forceinline__ bool test_bar(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
 // A whole warp's wait, first without the suspending form (a barrier that is
-// ready already costs the least so). One that ran out is recorded where the
-// caller gave a word for it, and every later one is skipped.
+// ready already costs the least so; `ready`: a test_bar the caller made some
+// work ago). One that ran out is recorded where the caller gave a word for it,
+// and every later one is skipped.
 struct Waiter {
     uint32_t *err;
     bool failed = false;
-    __device__ void operator()(uint64_t *bar, uint32_t parity) {
+    __device__ void operator()(uint64_t *bar, uint32_t parity) { (*this)(bar, parity, test_bar(bar, parity)); }
+    __device__ void operator()(uint64_t *bar, uint32_t parity, bool ready) {
+        if (__all_sync(0xffffffffu, ready) || failed) return;
         const uint32_t a = smem_u32(bar);
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (__all_sync(0xffffffffu, done) || failed) return;
         for (int i = 0; i < kPoll; ++i) {
+            uint32_t done;
             asm volatile(
                 "{\n\t.reg .pred p;\n\t"
                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -114,17 +120,14 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
     else
         tc_commit(bar);
 }
-// An arrival on this CTA's barrier (PAIR: on the leader's)
-template <bool PAIR>
-__device__ __forceinline__ void arrive(uint64_t *bar) {
-    if (PAIR)
-        asm volatile(
-            "{\n\t.reg .b32 r;\n\t"
-            "mapa.shared::cluster.u32 r, %0, 0;\n\t"
-            "mbarrier.arrive.shared::cluster.b64 _, [r];\n\t}\n" ::"r"(smem_u32(bar))
-            : "memory");
-    else
-        mbar_arrive(bar);
+__device__ __forceinline__ uint32_t map_cluster(uint32_t saddr, int cta) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(saddr), "r"(cta));
+    return r;
+}
+// An arrival on a barrier of the cluster (an address from map_cluster)
+__device__ __forceinline__ void arrive_at(uint32_t addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
 }
 template <bool PAIR>
 __device__ __forceinline__ bool rank_issues(int rank) {
@@ -155,6 +158,12 @@ __device__ __forceinline__ void fma2(uint64_t &d, uint64_t v, uint64_t s) {
 __device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
+__device__ __forceinline__ int ld_here(const int *p) {   // not sunk to its use
+    int v;
+    asm volatile("ld.global.nc.s32 %0, [%1];\n" : "=r"(v) : "l"(p));
+    return v;
+}
+
 // One lane of the (converged) warp. The roles that issue copies and MMAs run
 // their loops with the whole warp and elect a lane for the issue alone: the
 // loop stays uniform, so descriptors and barriers are built in uniform
@@ -174,11 +183,6 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 }
 __device__ __forceinline__ void cluster_arrive_wait() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ uint32_t map_cluster(uint32_t saddr, int cta) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(saddr), "r"(cta));
-    return r;
 }
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
     float v;
@@ -278,7 +282,7 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
 
 // ------------------------------------------------------------- the kernel
 
-enum Mode { kSingle = 0, kSplit = 1, kPair = 2 };
+enum Mode { kSingle = 0, kSplit = 1, kPair = 2, kSmall = 3 };
 
 constexpr int kAccCols = 256;                  // accumulator columns: two halves of 128
 constexpr int kThreads = 384;                  // TMA, MMA, two idle warps, eight epilogue warps
@@ -301,7 +305,6 @@ __device__ __forceinline__ uint32_t glu_pair(float g0, float g1, float u0, float
 // What the launcher fixes beyond GmmArgs.
 struct Plan {
     int bm;              // token rows a CTA loads for a tile (32, 64 or 128)
-    int box;             // weight rows of one TMA copy (256, 128 or 64)
     int stages;
     int split;           // kSplit: CTAs of a cluster
     int weights_first;   // the first stages' weights may be read before the kernel's predecessor has finished
@@ -469,19 +472,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
+            // every stage released: no commit is on its way when the CTA leaves
+            for (int i = 0; i < stages; ++i) {
+                wait(&empty[s], phase);
+                if (++s == stages) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
         } else if (warp == 1 && rank_issues<PAIR>(rank)) {
             // ---- MMA issuer: the sum of one scale block (e4m3) or of a tile
-            // (bf16) at a time
+            // (bf16) at a time. (In two halves of 128 columns, so that four
+            // smaller buffers hide the epilogue's answer, the MMAs themselves
+            // took 1.25 times as long.)
             constexpr uint32_t idesc = idesc_of(FP8, PAIR ? 256 : 128, kAccCols);
             int s = 0;
             uint32_t phase = 0, u = 0, uphase = 1;
             for (int tile = first; tile < tiles; tile += step) {
                 for (int kb = kb0; kb < kb1; ++kb) {
                     const bool fresh = FP8 || kb == kb0, last = FP8 || kb == kb1 - 1;
+                    const uint32_t st = sbase + s * stage_bytes, d = tmem + u * kAccCols;
                     wait(&full[s], phase);
                     if (fresh) wait(&acc_empty[u], uphase);
                     tc_fence_after();
-                    const uint32_t st = sbase + s * stage_bytes, d = tmem + u * kAccCols;
                     if (elect_one()) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
@@ -559,8 +572,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool busy = 32 * q < bm;              // lanes that hold token rows at all
         uint8_t *const patch = smem_raw + (sbase - smem_u32(smem_raw)) + kRingBytes + (warp - 4) * kPatch;
         const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + half * 128;
+        // the accumulators' barriers for the MMA issuer, a pair's in its leader
+        const uint32_t done0 = map_cluster(smem_u32(&acc_empty[0]), 0);
         uint32_t un = 0, sphase = 0;
         int slot = 0;
+        bool ready = false;
         for (int tile = first; tile < tiles; tile += step) {
             const Tile t = locate(a, s_g, tile, ntiles, tile_rows);
             const int r = t.row0 + (PAIR ? kLanes * rank : 0) + row;
@@ -571,6 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 64; ++j) acc[j] = 0;
             }
+            int orow = live ? r : -1;               // its output row
+            if (!GLU && !SPLIT && a.map && live) orow = ld_here(a.map + r);
             const int units = FP8 ? kb1 - kb0 : 1;
             for (int i0 = 0; i0 < units; i0 += kGroup) {
                 if (FP8) wait(&sc_full[slot], sphase);
@@ -588,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     const uint32_t u = un & 1, td = tq + u * kAccCols;
-                    wait(&acc_full[u], (un >> 1) & 1);
+                    wait(&acc_full[u], (un >> 1) & 1, ready);
                     ++un;
                     tc_fence_after();
                     uint32_t dv[2][32];
@@ -610,9 +628,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_ld32(td + 96, dv[1]);
                         tmem_wait_ld();
                     }
+                    // (every lane's tcgen05.ld is done: the wait is the warp's)
                     tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive<PAIR>(&acc_empty[u]);
+                    if (lane == 0) {
+                        if (PAIR) arrive_at(done0 + 8 * u);
+                        else mbar_arrive(&acc_empty[u]);
+                    }
+                    ready = test_bar(&acc_full[un & 1], (un >> 1) & 1);
                     if (busy) {
                         add(2);
                         add(3);
@@ -670,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 rows.flush(a.q_out + n0, a.N, live ? r : -1, a.N - n0);
                 if (half == 0 && live) a.s_out[(size_t)t.nt * a.P + r] = qs.s;
             } else {
-                const int o = live ? (a.map ? a.map[r] : r) : -1;
+                const int o = orow;
                 const RowStore<8> rows{patch, lane};
                 if (a.out_f32) {
                     uint8_t *y = reinterpret_cast<uint8_t *>(static_cast<float *>(a.out) + n0);
@@ -799,6 +821,284 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// ------------------------------------------ few tokens: weights on the lanes
+
+// Groups of a few tokens leave most of a 128-token tile's lanes empty, and its
+// two wide accumulators leave the tensor core waiting on the epilogue of a
+// tile of a few blocks. Here 128 weight rows take the lanes and 32 tokens are
+// the MMA's N: eight accumulators fit, all the lanes carry results, and the
+// two epilogue warpgroups take alternate tiles, so that one stores while the
+// other adds up. Each has its own accumulators and scale slots: a barrier's
+// parity tells two phases apart, so whoever waits on one has to see them all.
+// What bounds the kernel is the weights' stream from HBM.
+constexpr int kTok = 32;
+constexpr int kUnits = 4;                      // accumulators of a warpgroup
+constexpr int kSmallSlots = 2;                 // slots of staged scales of a warpgroup
+constexpr int kSmallRing = 184 * 1024;
+constexpr size_t kSmallSmem = 1024 + kSmallRing;
+
+template <int NMAT, bool FP8>
+__global__ void __launch_bounds__(kThreads, 1)
+    gmm_small_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw0,
+                     const __grid_constant__ CUtensorMap tw1, const GmmArgs a, const Plan p) {
+    constexpr bool GLU = NMAT == 2;
+    constexpr int kStageBytes = NMAT * 16384 + kTok * 128, kStages = kSmallRing / kStageBytes;
+    constexpr int kCols = NMAT * kTok, kAlloc = 2 * kUnits * kCols;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full[2][kUnits], acc_empty[2][kUnits];
+    __shared__ uint64_t sc_full[2][kSmallSlots], sc_empty[2][kSmallSlots];
+    __shared__ uint32_t s_tmem;
+    __shared__ Groups s_g;
+    // products of token and weight scales: [warpgroup][slot][block][matrix][token]
+    __shared__ __align__(16) float s_scale[FP8 ? 2 * kSmallSlots * kGroup * kCols : 4];
+    __shared__ __align__(16) uint16_t s_out[2][kTok * kLanes];      // [warpgroup][token][weight row]
+    __shared__ uint32_t s_amax[GLU ? 2 : 1][4][kTok];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2 * kUnits; ++i) {
+            mbar_init(&acc_full[i / kUnits][i % kUnits], 1);
+            mbar_init(&acc_empty[i / kUnits][i % kUnits], 4);
+        }
+        for (int i = 0; i < 2 * kSmallSlots; ++i) {
+            mbar_init(&sc_full[i / kSmallSlots][i % kSmallSlots], NMAT);
+            mbar_init(&sc_empty[i / kSmallSlots][i % kSmallSlots], 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)),
+                     "r"(kAlloc)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    pdl_wait();
+    pdl_trigger();
+    if (a.off && warp == 0) build_groups(a, s_g, kTok);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const int ntiles = (a.N + kLanes - 1) / kLanes;
+    const int tiles = (a.off ? s_g.pre[a.E] : (a.P + kTok - 1) / kTok) * ntiles;
+    const int units = FP8 ? a.KB : 1;              // accumulators of a tile
+    Waiter wait{a.err};
+    if (warp == 0) {
+        // ---- TMA producer
+        int s = 0;
+        uint32_t phase = 1;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            const Tile t = locate(a, s_g, tile, ntiles, kTok);
+            const int wrow = t.e * a.N + t.nt * kLanes;
+            for (int kb = 0; kb < a.KB; ++kb) {
+                const uint32_t st = sbase + s * kStageBytes;
+                wait(&empty[s], phase);
+                if (elect_one()) {
+                    arrive_expect_tx(&full[s], kStageBytes);
+                    tma_load_2d(st, &tw0, kb * 128, wrow, &full[s]);
+                    if (GLU) tma_load_2d(st + 16384, &tw1, kb * 128, wrow, &full[s]);
+                    tma_load_2d(st + NMAT * 16384, &tx, kb * 128, t.row0, &full[s]);
+                }
+                __syncwarp();
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        // every stage released: no commit is on its way when the CTA leaves
+        for (int i = 0; i < kStages; ++i) {
+            wait(&empty[s], phase);
+            if (++s == kStages) {
+                s = 0;
+                phase ^= 1;
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer
+        constexpr uint32_t idesc = idesc_of(FP8, kLanes, kTok);
+        int s = 0, wg = 0;
+        uint32_t phase = 0, un[2] = {0, 0};        // accumulators handed to each warpgroup
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, wg ^= 1) {
+            uint32_t c = wg ? un[1] : un[0];
+            for (int kb = 0; kb < a.KB; ++kb) {
+                const bool fresh = FP8 || kb == 0, last = FP8 || kb == a.KB - 1;
+                const uint32_t u = c % kUnits, d = tmem + (wg * kUnits + u) * kCols;
+                const uint32_t st = sbase + s * kStageBytes;
+                wait(&full[s], phase);
+                if (fresh) wait(&acc_empty[wg][u], ((c / kUnits) & 1) ^ 1);
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int m = 0; m < NMAT; ++m)
+                            mma_ss<FP8, false>(d + m * kTok, sw128_desc(st + m * 16384 + 32 * q),
+                                               sw128_desc(st + NMAT * 16384 + 32 * q), idesc, !fresh || q > 0);
+                    tc_commit(&empty[s]);
+                    if (last) tc_commit(&acc_full[wg][u]);
+                }
+                __syncwarp();
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1;
+                }
+                if (last) ++c;
+            }
+            if (wg) un[1] = c;
+            else un[0] = c;
+        }
+    } else if (warp < 4) {
+        // ---- scales: a warp a matrix, a lane a token
+        if (FP8 && warp - 2 < NMAT) {
+            const int m = warp - 2;
+            int wg = 0;
+            uint32_t gg[2] = {0, 0};               // slots filled for each warpgroup
+            for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, wg ^= 1) {
+                uint32_t g = wg ? gg[1] : gg[0];
+                const Tile t = locate(a, s_g, tile, ntiles, kTok);
+                const float *w = (m ? a.sw1 : a.sw0) + ((size_t)t.e * ntiles + t.nt) * a.KB;
+                const float *x = a.sx + min(t.row0 + lane, a.P - 1);
+                for (int i0 = 0; i0 < units; i0 += kGroup, ++g) {
+                    const uint32_t slot = g % kSmallSlots;
+                    float v[kGroup], f[kGroup];
+#pragma unroll
+                    for (int z = 0; z < kGroup; ++z) {
+                        const int i = min(i0 + z, units - 1);
+                        v[z] = __ldg(x + (size_t)i * a.P);
+                        f[z] = __ldg(w + i);
+                    }
+                    wait(&sc_empty[wg][slot], ((g / kSmallSlots) & 1) ^ 1);
+#pragma unroll
+                    for (int z = 0; z < kGroup; ++z)
+                        s_scale[(((wg * kSmallSlots + slot) * kGroup + z) * NMAT + m) * kTok + lane] = v[z] * f[z];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_full[wg][slot]);
+                }
+                if (wg) gg[1] = g;
+                else gg[0] = g;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- epilogue: thread = one weight row; the warpgroups take alternate tiles
+        const int wg = (warp - 4) >> 2, q = warp & 3, row = 32 * q + lane;
+        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + wg * kUnits * kCols;
+        uint32_t un = 0, gg = 0;                    // accumulators and scale slots this warpgroup has read
+        uint16_t *const so = s_out[wg];
+        for (int tile = blockIdx.x + wg * gridDim.x; tile < tiles; tile += 2 * gridDim.x) {
+            const Tile t = locate(a, s_g, tile, ntiles, kTok);
+            const int np = min(kTok, t.end - t.row0), n0 = t.nt * kLanes, n = n0 + row;
+            // lane's token: its output row
+            int orow = -1;
+            if (lane < np) orow = !GLU && a.map ? ld_here(a.map + t.row0 + lane) : t.row0 + lane;
+            uint64_t acc[NMAT][kTok / 2];
+#pragma unroll
+            for (int m = 0; m < NMAT; ++m)
+#pragma unroll
+                for (int j = 0; j < kTok / 2; ++j) acc[m][j] = 0;
+            for (int i0 = 0; i0 < units; i0 += kGroup, ++gg) {
+                const uint32_t slot = gg % kSmallSlots;
+                if (FP8) wait(&sc_full[wg][slot], (gg / kSmallSlots) & 1);
+                for (int i = i0; i < min(i0 + kGroup, units); ++i, ++un) {
+                    const uint32_t u = un % kUnits;
+                    wait(&acc_full[wg][u], (un / kUnits) & 1);
+                    tc_fence_after();
+                    uint32_t dv[NMAT][32];
+#pragma unroll
+                    for (int m = 0; m < NMAT; ++m) tmem_ld32(tq + u * kCols + m * kTok, dv[m]);
+                    tmem_wait_ld();
+                    tc_fence_before();
+                    if (lane == 0) mbar_arrive(&acc_empty[wg][u]);
+#pragma unroll
+                    for (int m = 0; m < NMAT; ++m) {
+                        const ulonglong2 *sc = reinterpret_cast<const ulonglong2 *>(
+                            s_scale + (((wg * kSmallSlots + slot) * kGroup + i - i0) * NMAT + m) * kTok);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            if (FP8) {
+                                const ulonglong2 s = sc[j];
+                                fma2(acc[m][2 * j], pack2(dv[m][4 * j], dv[m][4 * j + 1]), s.x);
+                                fma2(acc[m][2 * j + 1], pack2(dv[m][4 * j + 2], dv[m][4 * j + 3]), s.y);
+                            } else {
+                                acc[m][2 * j] = pack2(dv[m][4 * j], dv[m][4 * j + 1]);
+                                acc[m][2 * j + 1] = pack2(dv[m][4 * j + 2], dv[m][4 * j + 3]);
+                            }
+                        }
+                    }
+                }
+                if (FP8) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_empty[wg][slot]);
+                }
+            }
+            if (!GLU && a.out_f32) {
+#pragma unroll
+                for (int j = 0; j < kTok; ++j) {
+                    const int o = __shfl_sync(0xffffffffu, orow, j);
+                    const float v = j & 1 ? hi2(acc[0][j >> 1]) : lo2(acc[0][j >> 1]);
+                    if (o >= 0 && n < a.N) static_cast<float *>(a.out)[o * a.out_stride + n] = v;
+                }
+                continue;
+            }
+            const float rs = !GLU && a.row_scale && orow >= 0 ? a.row_scale[orow] : 1.0f;
+            uint32_t most = 0;
+#pragma unroll
+            for (int j = 0; j < kTok / 2; ++j) {
+                uint32_t w;
+                if (GLU) {
+                    w = glu_pair(lo2(acc[0][j]), hi2(acc[0][j]), lo2(acc[NMAT - 1][j]), hi2(acc[NMAT - 1][j]), a.act);
+                    const uint32_t m = n < a.N ? w & 0x7FFF7FFFu : 0u;
+                    const uint32_t m0 = __reduce_max_sync(0xffffffffu, m & 0xFFFFu);
+                    const uint32_t m1 = __reduce_max_sync(0xffffffffu, m >> 16);
+                    if (lane == 2 * j) most = m0;
+                    if (lane == 2 * j + 1) most = m1;
+                } else {
+                    w = cvt_bf16x2(lo2(acc[0][j]), hi2(acc[0][j]));
+                    if (a.row_scale)
+                        w = cvt_bf16x2(bf_lo(w) * __shfl_sync(0xffffffffu, rs, 2 * j),
+                                       bf_hi(w) * __shfl_sync(0xffffffffu, rs, 2 * j + 1));
+                }
+                so[2 * j * kLanes + row] = (uint16_t)w;
+                so[(2 * j + 1) * kLanes + row] = (uint16_t)(w >> 16);
+            }
+            if (GLU) s_amax[GLU ? wg : 0][q][lane] = most;
+            bar_sync(1 + wg, 128);
+            // eight tokens a warp, sixteen lanes a token's 128 values
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int tok = 8 * q + 2 * k + (lane >> 4), c = 8 * (lane & 15);
+                const int o = __shfl_sync(0xffffffffu, orow, tok);
+                if (o < 0 || n0 + c >= a.N) continue;
+                const uint4 v = *reinterpret_cast<const uint4 *>(so + tok * kLanes + c);
+                if (GLU) {
+                    const uint32_t *am = &s_amax[GLU ? wg : 0][0][tok];
+                    const QScale qs = qscale(max(max(am[0], am[kTok]), max(am[2 * kTok], am[3 * kTok])));
+                    const uint32_t lo = cvt_e4m3x2(quotient(bf_lo(v.x), qs), quotient(bf_hi(v.x), qs)) |
+                                        (cvt_e4m3x2(quotient(bf_lo(v.y), qs), quotient(bf_hi(v.y), qs)) << 16);
+                    const uint32_t hi = cvt_e4m3x2(quotient(bf_lo(v.z), qs), quotient(bf_hi(v.z), qs)) |
+                                        (cvt_e4m3x2(quotient(bf_lo(v.w), qs), quotient(bf_hi(v.w), qs)) << 16);
+                    *reinterpret_cast<uint2 *>(a.q_out + (size_t)o * a.N + n0 + c) = make_uint2(lo, hi);
+                    if (c == 0) a.s_out[(size_t)t.nt * a.P + o] = qs.s;
+                } else {
+                    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + o * a.out_stride + n0 + c) = v;
+                }
+            }
+            bar_sync(1 + wg, 128);                  // read before this warpgroup's next tile
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kAlloc) : "memory");
+    }
+}
+
 // ---------------------------------------------------------------- host
 
 // The epilogue warps take registers that the block's other warps gave up. A
@@ -827,6 +1127,36 @@ static bool byte_map(CUtensorMap *m, const void *base, size_t rows, size_t row_b
     return encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, dims, pitch, box) == CUDA_SUCCESS;
 }
 
+// How many clusters of `size` CTAs of the kernel run at a time (each CTA takes
+// an SM, and a cluster stays inside one GPC), looked up once per device.
+static int max_clusters(const void *fn, int size) {
+    static std::mutex mu;
+    static std::map<std::pair<int, int>, int> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = known.find({dev, size});
+    if (it != known.end()) return it->second;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (ensure_dynamic_smem(fn, kSmem, "gmm_kernel") != VQMOE_OK ||
+        cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+    }
+    known[{dev, size}] = n;
+    return n;
+}
+
 template <int MODE>
 static const void *kernel_of(bool glu, bool fp8) {
     return glu   ? reinterpret_cast<const void *>(&gmm_kernel<true, true, MODE>)
@@ -846,48 +1176,93 @@ vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const voi
     if ((long long)a.E * a.N > 0x7FFFFFFFLL - 256 || (long long)a.KB * 128 > 0x7FFFFFFFLL)
         return set_error(VQMOE_BAD_SHAPE, "grouped product: %d groups of %d rows", a.E, a.N);
     const int sms = sm_count();
-    // groups that can have rows, their mean rows, and (a bound on) the tiles of `rows` token rows
-    const int groups = std::min(a.E, a.P), mean = (a.P + groups - 1) / groups;
+    // groups that can have rows, and the tiles of `rows` token rows (a bound, with ragged groups)
+    const int groups = std::min(a.E, a.P);
     const long long ntiles = (a.N + (glu ? 127 : 255)) / (glu ? 128 : 256);
     auto tiles_of = [&](int rows) {
         return ntiles * (a.off ? std::min<long long>(a.P, a.P / rows + groups) : (a.P + rows - 1) / rows);
     };
+    // Which mode: the least estimated time, waves of tiles times their blocks,
+    // from measured microseconds of a 128-byte block, a tile's other work and,
+    // for a split tile, bringing the sums together (fixed, and by its rows).
+    const int small_cols = (int)(((a.N + kLanes - 1) / kLanes + ntiles - 1) / ntiles);   // kSmall's column tiles of one here
+    const double unit = fp8 ? 1.0 : 0.8;
     Plan p{};
-    p.bm = mean <= 24 ? 32 : mean <= 48 ? 64 : 128;
-    p.split = 1;
-    const char *env = getenv("GMM_MODE");
-    int mode = mean > 128 ? kPair : kSingle;
-    if (env) mode = atoi(env);
-    if (const char *b = getenv("GMM_BM")) p.bm = atoi(b);
-    if (mode != kPair) {
-        while (p.split < 8 && tiles_of(p.bm) * p.split * 2 <= sms && p.split * 4 <= a.KB) p.split *= 2;
-        mode = p.split > 1 ? kSplit : kSingle;
+    int mode = kSingle;
+    double best = 1e30;
+    auto consider = [&](int m, int bm, int split, double block, double other, int slots) {
+        const long long tiles = tiles_of(m == kPair ? 2 * bm : bm) * (m == kSmall ? small_cols : 1);
+        const double cost = (double)((tiles + slots - 1) / slots) * ((a.KB + split - 1) / split * block * unit + other);
+        if (cost < best) {
+            best = cost;
+            mode = m;
+            p.bm = bm;
+            p.split = split;
+        }
+    };
+    if (a.off) {
+        // Ragged: the host knows the mean alone, so the tile goes by that.
+        // Measured at 128 groups of 768 x 2048 (us; kSmall / kSingle with 64 /
+        // with 128 rows / kPair), even and Zipf-distributed groups: mean 4
+        // e4m3 42 / 46 / 48 / 69 and 37 / 45 / 46 / 58, bf16 70 / 68 / 71 / 86
+        // and 58 / 65 / 69 / 68; mean 16 e4m3 47 / 50 / 52 and 50 / 50 / 51,
+        // bf16 73 / 71 / 74 and 80 / 70 / 73; mean 32 e4m3 56 / 53 / 55 and 63 /
+        // 63 / 53; mean 256 (128 rows / kPair) e4m3 132 / 134, bf16 147 / 136;
+        // mean 512 e4m3 229 / 228, bf16 241 / 210. e4m3 gate/up and down: mean
+        // 32 150 / 190 / 196, mean 64 219 / 238 / 207, mean 512 692 / 709.
+        const int mean = (a.P + groups - 1) / groups;
+        if (mean <= (glu ? 40 : fp8 ? 20 : 6)) consider(kSmall, kTok, 1, glu ? 0.74 : 0.37, 0.7, sms);
+        else if (mean <= 24) consider(kSingle, 64, 1, 0.55, 3.0, sms);
+        else if (mean < (fp8 ? 640 : 192)) consider(kSingle, 128, 1, 0.6, 3.0, sms);
+        else consider(kPair, 128, 1, 0.6, 3.0, sms / 2);
     } else {
-        p.bm = kLanes;
+        consider(kPair, 128, 1, 0.58, 2.0, sms / 2);
+        consider(kSingle, 128, 1, 0.60, 2.0, sms);
+        consider(kSingle, 64, 1, 0.55, 2.0, sms);
+        consider(kSingle, 32, 1, 0.45, 2.0, sms);
     }
+    // Splitting pays while a wave of tiles leaves SMs idle: one wave of clusters
+    // then, at least two blocks a CTA. (4096 x 4096 e4m3, one token: 1 x 16
+    // CTAs 19.5 us, clusters of 4 11.5, of 6 10.7, of 8, which do not all fit at
+    // once, 18.)
+    for (int bm = 32; bm <= 128; bm *= 2)
+        for (int s = 2; s <= 8 && 2 * s <= a.KB; ++s)
+            if (tiles_of(bm) * s <= sms) {
+                const int slots = max_clusters(kernel_of<kSplit>(glu, fp8), s);
+                if (tiles_of(bm) <= slots)
+                    consider(kSplit, bm, s, bm == 32 ? 0.45 : bm == 64 ? 0.5 : 0.55,
+                             3.5 + 0.01 * bm + 0.1 * bm / s, slots);
+            }
     const int stage = p.bm * 128 + (mode == kPair ? 128 : 256) * 128;
     p.stages = std::min(kMaxStages, kRingBytes / stage);
-    p.box = glu ? 64 : mode == kPair ? 128 : 256;
+    const int box = mode == kSmall ? kLanes : glu ? 64 : mode == kPair ? 128 : 256;
     p.weights_first = pdl_weights && !a.off && mode != kPair;
     const int cluster = mode == kPair ? 2 : p.split;
-    const long long tiles = std::min<long long>(tiles_of(mode == kPair ? 256 : p.bm), 1 << 20);
+    const long long tiles = std::min<long long>(tiles_of(mode == kPair ? 256 : p.bm) * (mode == kSmall ? small_cols : 1),
+                                                1 << 20);
     const int grid = mode == kSplit ? (int)tiles * p.split
                      : mode == kPair ? 2 * (int)std::min<long long>(tiles, sms / 2)
                                      : (int)std::min<long long>(tiles, sms);
     CUtensorMap mx, m0, m1;
     const size_t wrows = (size_t)a.E * a.N;
-    if (!byte_map(&mx, x, a.P, row_bytes, x_pitch, p.bm) || !byte_map(&m0, w0, wrows, row_bytes, row_bytes, p.box) ||
-        !byte_map(&m1, glu ? w1 : w0, wrows, row_bytes, row_bytes, p.box))
+    if (!byte_map(&mx, x, a.P, row_bytes, x_pitch, p.bm) || !byte_map(&m0, w0, wrows, row_bytes, row_bytes, box) ||
+        !byte_map(&m1, glu ? w1 : w0, wrows, row_bytes, row_bytes, box))
         return set_error(VQMOE_LAUNCH_FAILED, "grouped product: tensor map");
     const void *fn = mode == kPair    ? kernel_of<kPair>(glu, fp8)
                      : mode == kSplit ? kernel_of<kSplit>(glu, fp8)
+                     : mode == kSmall ? (glu   ? reinterpret_cast<const void *>(&gmm_small_kernel<2, true>)
+                                         : fp8 ? reinterpret_cast<const void *>(&gmm_small_kernel<1, true>)
+                                               : reinterpret_cast<const void *>(&gmm_small_kernel<1, false>))
                                       : kernel_of<kSingle>(glu, fp8);
-    vqmoe_status s = check_registers(fn);
-    if (s != VQMOE_OK || (s = ensure_dynamic_smem(fn, kSmem, "gmm_kernel")) != VQMOE_OK) return s;
+    const size_t smem = mode == kSmall ? kSmallSmem : kSmem;
+    vqmoe_status s;
+    if ((mode != kSmall && (s = check_registers(fn)) != VQMOE_OK) ||
+        (s = ensure_dynamic_smem(fn, smem, "gmm_kernel")) != VQMOE_OK)
+        return s;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmem;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -906,53 +1281,82 @@ vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const voi
 
 namespace gm {
 
-// A half warp per group of 128: 8 values a lane, the largest |bf16| by
-// integer comparison of the bits (a NaN compares above an infinity, and both
-// above every finite value).
+// Eight lanes a group of 128, 16 values each; a thread has kQuantAhead groups'
+// loads in flight (a row's bytes are read and written once: HBM-bound). The
+// largest |bf16| by integer comparison of the bits: a NaN compares above an
+// infinity, and both above every finite value.
+constexpr int kQuantAhead = 2;
 template <bool ORDER>
 __global__ void __launch_bounds__(256)
-    quantize_kernel(const uint16_t *__restrict__ x, long long rows, int cols, long long x_stride,
+    quantize_kernel(const uint16_t *__restrict__ x, uint32_t total, uint32_t groups, int cols, long long x_stride,
                     uint8_t *__restrict__ q, float *__restrict__ s, long long s_row, long long s_group,
                     const QuantOrder o) {
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 15;
-    const int groups = (cols + kScaleBlock - 1) / kScaleBlock;
-    const long long total = rows * groups, half = (long long)gridDim.x * 16;
-    // every lane of a warp runs the same trips (the shuffles need both halves)
-    const long long h0 = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const long long trips = (total + half - 1) / half;
-    for (long long i = 0; i < trips; ++i) {
-        const long long g = h0 + i * half;
-        const bool in = g < total;
-        const long long row = in ? g / groups : 0;
-        const int grp = in ? (int)(g - row * groups) : 0;
-        const int c = grp * kScaleBlock + lane * 8;
-        const bool live = in && c < cols;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live) v = __ldg(reinterpret_cast<const uint4 *>(x + row * x_stride + c));
-        uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
-                              __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+    const int lane = threadIdx.x & 7;
+    const uint32_t slots = gridDim.x * 32, slot = blockIdx.x * 32 + (threadIdx.x >> 3);
+    // every lane of a warp makes the same trips (the shuffles need all of them)
+    const uint32_t trips = (total + slots - 1) / slots;
+    for (uint32_t i0 = 0; i0 < trips; i0 += kQuantAhead) {
+        uint4 v[kQuantAhead][2];
+        uint32_t row[kQuantAhead];
+        int c[kQuantAhead];
+        bool in[kQuantAhead];
 #pragma unroll
-        for (int d = 8; d > 0; d >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const QScale qs = qscale(max(m & 0xFFFFu, m >> 16));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint32_t b[4];
+        for (int z = 0; z < kQuantAhead; ++z) {
+            const uint32_t g = slot + (i0 + z) * slots;
+            in[z] = i0 + z < trips && g < total;
+            row[z] = in[z] ? g / groups : 0;
+            c[z] = in[z] ? (int)(g - row[z] * groups) * kScaleBlock + lane * 16 : 0;
+            v[z][0] = v[z][1] = make_uint4(0, 0, 0, 0);
+            if (in[z] && c[z] < cols) {
+                const uint4 *p = reinterpret_cast<const uint4 *>(x + row[z] * x_stride + c[z]);
+                v[z][0] = __ldcs(p);
+                v[z][1] = __ldcs(p + 1);
+            }
+        }
 #pragma unroll
-        for (int z = 0; z < 4; ++z) b[z] = cvt_e4m3x2(quotient(bf_lo(w[z]), qs), quotient(bf_hi(w[z]), qs));
-        const uint2 r = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
-        if (!ORDER) {
-            if (live) *reinterpret_cast<uint2 *>(q + row * cols + c) = r;
-            if (in && lane == 0) s[row * s_row + grp * s_group] = qs.s;
-        } else if (in) {
-            const int k = o.per_pair ? 1 : o.k;
-            for (int z = 0; z < k; ++z) {
-                const long long p = row * k + z;
-                const int rk = __ldg(o.rank + p);
-                if (rk < 0) continue;               // no such expert: the pair has no place
-                const long long at = __ldg(o.off + __ldg(o.inds + p)) + rk;
-                if (live) *reinterpret_cast<uint2 *>(q + at * cols + c) = r;
-                if (lane == 0) s[at * s_row + grp * s_group] = qs.s;
+        for (int z = 0; z < kQuantAhead; ++z) {
+            const uint32_t w[8] = {v[z][0].x, v[z][0].y, v[z][0].z, v[z][0].w,
+                                   v[z][1].x, v[z][1].y, v[z][1].z, v[z][1].w};
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+#pragma unroll
+            for (int d = 4; d > 0; d >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const QScale qs = qscale(max(m & 0xFFFFu, m >> 16));
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                b[j] = cvt_e4m3x2(quotient(bf_lo(w[2 * j]), qs), quotient(bf_hi(w[2 * j]), qs)) |
+                       (cvt_e4m3x2(quotient(bf_lo(w[2 * j + 1]), qs), quotient(bf_hi(w[2 * j + 1]), qs)) << 16);
+            if (!in[z]) continue;
+            const uint4 r = make_uint4(b[0], b[1], b[2], b[3]);
+            const bool live = c[z] < cols;
+            const long long grp = c[z] / kScaleBlock;
+            if (!ORDER) {
+                if (live) *reinterpret_cast<uint4 *>(q + (size_t)row[z] * cols + c[z]) = r;
+                if (lane == 0) s[row[z] * s_row + grp * s_group] = qs.s;
+            } else {
+                // the places of the row's pairs, eight looked up at a time
+                const int k = o.per_pair ? 1 : o.k;
+                for (int y0 = 0; y0 < k; y0 += 8) {
+                    int rk[8], at[8];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        const size_t p = (size_t)row[z] * k + min(y0 + y, k - 1);
+                        rk[y] = y0 + y < k ? __ldg(o.rank + p) : -1;      // < 0: no such expert, no place
+                        at[y] = rk[y] >= 0 ? __ldg(o.inds + p) : 0;
+                    }
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) at[y] = rk[y] >= 0 ? __ldg(o.off + at[y]) + rk[y] : -1;
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        if (at[y] < 0) continue;
+                        if (live) *reinterpret_cast<uint4 *>(q + (size_t)at[y] * cols + c[z]) = r;
+                        if (lane == 0) s[at[y] * s_row + grp * s_group] = qs.s;
+                    }
+                }
             }
         }
     }
@@ -963,15 +1367,22 @@ __global__ void __launch_bounds__(256)
 vqmoe_status launch_quantize_fp8(const void *x, long long rows, int cols, long long x_stride, uint8_t *q, float *s,
                                  long long s_row, long long s_group, const QuantOrder *order, cudaStream_t stream) {
     if (rows <= 0) return VQMOE_OK;
-    const long long groups = rows * ((cols + kScaleBlock - 1) / kScaleBlock);
-    const int grid = (int)std::min<long long>((groups + 15) / 16, (long long)sm_count() * 16);
+    const uint32_t groups = (cols + kScaleBlock - 1) / kScaleBlock;
+    const long long total = rows * groups;
+    if (total > 0x7FFFFFFFLL) return set_error(VQMOE_BAD_SHAPE, "quantize: %lld rows of %d", rows, cols);
+    const int grid = (int)std::min<long long>((total + 31) / 32, (long long)sm_count() * 8);
     const uint16_t *xp = static_cast<const uint16_t *>(x);
-    if (order)
-        gm::quantize_kernel<true><<<grid, 256, 0, stream>>>(xp, rows, cols, x_stride, q, s, s_row, s_group, *order);
-    else
-        gm::quantize_kernel<false><<<grid, 256, 0, stream>>>(xp, rows, cols, x_stride, q, s, s_row, s_group, QuantOrder{});
+    if (order) {
+        if (launch_pdl(gm::quantize_kernel<true>, dim3(grid), dim3(256), 0, stream, xp, (uint32_t)total, groups, cols,
+                       x_stride, q, s, s_row, s_group, *order) != cudaSuccess)
+            return check_launch("quantize_kernel");
+        return VQMOE_OK;
+    }
+    gm::quantize_kernel<false><<<grid, 256, 0, stream>>>(xp, (uint32_t)total, groups, cols, x_stride, q, s, s_row,
+                                                         s_group, QuantOrder{});
     return check_launch("quantize_kernel");
 }
+
 
 // ---------------------------------------------- routed experts, C ABI
 

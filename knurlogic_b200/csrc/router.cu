@@ -808,6 +808,91 @@ vqmoe_status launch_route(const int32_t *inds, int P, int E, int32_t *cnt,
     return check_launch("route_kernel");
 }
 
+// The same sort spread over CTAs, for many pairs (one CTA takes 35 us for
+// 32768 pairs, its shared-memory atomics and its two passes over them; these
+// two launches 9): each CTA counts its pairs per expert in shared memory and
+// takes a run of places for each expert from the global count; then every CTA
+// scans the counts and places its pairs. cnt[0 .. E) zero on entry.
+constexpr int kRouteWideThreads = 512;
+constexpr int kRouteWidePairs = 512;          // pairs of a CTA
+__global__ void __launch_bounds__(kRouteWideThreads)
+route_count_kernel(const int32_t *__restrict__ inds, int P, int E, int32_t *__restrict__ cnt,
+                   int32_t *__restrict__ rank) {
+    __shared__ int32_t s_cnt[1024], s_base[1024];
+    const int tid = threadIdx.x;
+    for (int e = tid; e < E; e += kRouteWideThreads) s_cnt[e] = 0;
+    __syncthreads();
+    const int p = blockIdx.x * kRouteWidePairs + tid;
+    const int e = p < P ? inds[p] : -1;
+    const bool ok = e >= 0 && e < E;
+    const int r = ok ? atomicAdd(&s_cnt[e], 1) : -1;
+    __syncthreads();
+    for (int i = tid; i < E; i += kRouteWideThreads) s_base[i] = s_cnt[i] ? atomicAdd(cnt + i, s_cnt[i]) : 0;
+    __syncthreads();
+    if (p < P) rank[p] = ok ? s_base[e] + r : -1;
+}
+__global__ void __launch_bounds__(kRouteWideThreads)
+route_place_kernel(const int32_t *__restrict__ inds, int P, int E, const int32_t *__restrict__ cnt,
+                   int32_t *__restrict__ off, int32_t *__restrict__ list, int32_t *__restrict__ active,
+                   const int32_t *__restrict__ rank) {
+    __shared__ int32_t s_off[1024];
+    __shared__ int32_t s_wsum[kRouteWideThreads / 32], s_asum[kRouteWideThreads / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // two experts a thread: exclusive sums of the counts and of (count > 0)
+    const int e0 = 2 * tid, e1 = e0 + 1;
+    const int c0 = e0 < E ? cnt[e0] : 0, c1 = e1 < E ? cnt[e1] : 0;
+    int ic = c0 + c1, ia = (c0 > 0) + (c1 > 0);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, ic, o), v = __shfl_up_sync(0xffffffffu, ia, o);
+        if (lane >= o) {
+            ic += u;
+            ia += v;
+        }
+    }
+    if (lane == 31) {
+        s_wsum[warp] = ic;
+        s_asum[warp] = ia;
+    }
+    __syncthreads();
+    int oc = ic - c0 - c1, oa = ia - (c0 > 0) - (c1 > 0);
+    for (int w = 0; w < warp; ++w) {
+        oc += s_wsum[w];
+        oa += s_asum[w];
+    }
+    if (e0 < E) s_off[e0] = oc;
+    if (e1 < E) s_off[e1] = oc + c0;
+    if (blockIdx.x == 0) {
+        if (e0 < E) {
+            off[e0] = oc;
+            if (c0) active[oa] = e0;
+        }
+        if (e1 < E) {
+            off[e1] = oc + c0;
+            if (c1) active[oa + (c0 > 0)] = e1;
+        }
+        if (e0 == E - 1 || e1 == E - 1) {
+            off[E] = oc + c0 + c1;
+            active[E] = oa + (c0 > 0) + (c1 > 0);
+        }
+    }
+    __syncthreads();
+    const int p = blockIdx.x * kRouteWidePairs + tid;
+    if (p < P && rank[p] >= 0) list[s_off[inds[p]] + rank[p]] = p;
+}
+
+vqmoe_status launch_route_wide(const int32_t *inds, int P, int E, int32_t *cnt, int32_t *off, int32_t *list,
+                               int32_t *active, int32_t *rank, cudaStream_t stream) {
+    if (E > 1024) return set_error(VQMOE_BAD_SHAPE, "route: %d experts (<= 1024)", E);
+    if (cudaMemsetAsync(cnt, 0, (size_t)E * sizeof(int32_t), stream) != cudaSuccess) return check_launch("route counts");
+    const int grid = (P + kRouteWidePairs - 1) / kRouteWidePairs;
+    route_count_kernel<<<grid, kRouteWideThreads, 0, stream>>>(inds, P, E, cnt, rank);
+    vqmoe_status s = check_launch("route_count_kernel");
+    if (s != VQMOE_OK) return s;
+    route_place_kernel<<<grid, kRouteWideThreads, 0, stream>>>(inds, P, E, cnt, off, list, active, rank);
+    return check_launch("route_place_kernel");
+}
+
 // ------------------------------------------------------------ RMS norm
 // Gemma-4's router input, mx.fast.rms_norm(x, w, eps) (gemma4_text.py:
 // 171): out = bf16(bf16(x * r) * w), r = 1 / sqrt(ms + eps) in float32

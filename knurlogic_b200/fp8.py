@@ -19,7 +19,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .switch_layers import _contig, c_stream, check_fp8_weight, ctypes_ref, require_cuda
+from .switch_layers import _contig, c_stream, check_fp8_weight, fp8_descriptor, require_cuda
 
 GROUP = 128
 _status: dict = {}
@@ -50,18 +50,32 @@ def check_status(device=None) -> None:
 def _rows(x: torch.Tensor, features: int) -> torch.Tensor:
     """x as [rows, features] bf16 with unit stride along a row; a copy only
     where a row's pitch or start is not the kernels' (16 bytes)."""
-    if x.dtype != torch.bfloat16:
+    if not x.is_cuda:
+        require_cuda(x)
+    if x.dtype is not torch.bfloat16:
         raise TypeError(f"x must be bfloat16, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] != features:
         raise ValueError(f"x {tuple(x.shape)} has not {features} features")
-    x = x.reshape(-1, features)
-    if x.shape[0] and (x.stride(1) != 1 or x.stride(0) < features or x.stride(0) % 8 or x.data_ptr() % 16):
+    if x.dim() != 2:
+        x = x.reshape(-1, features)
+    pitch, one = x.stride()
+    if x.shape[0] and (one != 1 or pitch < features or pitch % 8 or x.data_ptr() % 16):
         x = x.contiguous() if not x.is_contiguous() else x.clone()
     return x
 
 
 def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """An entry point on `device` and its current stream (the last argument)."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        _lib.call(name, *args, c_stream(device))
+    else:
+        with torch.cuda.device(i):
+            _lib.call(name, *args, c_stream(device))
 
 
 def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -71,17 +85,14 @@ def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         scale = f32(a / 448),  q = e4m3(448 x / a)
     -- the exact quotient rounded once, ties to even. A NaN or an infinity in
     a group makes its scale NaN. K is a multiple of 16."""
-    require_cuda(x)
     K = x.shape[-1] if x.dim() else 0
     if K <= 0 or K % 16:
         raise ValueError(f"x {tuple(x.shape)}: the last dimension must be a multiple of 16")
     xr = _rows(x, K)
-    q = torch.empty((*x.shape[:-1], K), dtype=torch.float8_e4m3fn, device=x.device)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     s = torch.empty((*x.shape[:-1], -(-K // GROUP)), dtype=torch.float32, device=x.device)
     if xr.shape[0]:
-        with torch.cuda.device(x.device):
-            _lib.call("vqmoe_quantize_fp8", xr.data_ptr(), xr.shape[0], K, _pitch(xr), q.data_ptr(), s.data_ptr(),
-                      c_stream(x.device))
+        _call_on(x.device, "vqmoe_quantize_fp8", xr.data_ptr(), xr.shape[0], K, _pitch(xr), q.data_ptr(), s.data_ptr())
     return q, s
 
 
@@ -91,14 +102,15 @@ def _run(d: _lib.Linear, x: torch.Tensor, offsets, out: torch.Tensor) -> torch.T
     if P == 0:
         return out
     dev = x.device
-    with torch.cuda.device(dev):
-        n = _lib.lib().vqmoe_grouped_linear_workspace_size(ctypes_ref(d), P)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    n = _lib.lib().vqmoe_grouped_linear_workspace_size(d, P)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    st = _status.get(dev.index)
+    if st is None:
         st = _status_word(dev)
-        _lib.call("vqmoe_grouped_linear", ctypes_ref(d), x.data_ptr(), P, _pitch(x),
-                  offsets.data_ptr() if offsets is not None else None, out.data_ptr(),
-                  _lib.OUT_F32 if out.dtype == torch.float32 else _lib.OUT_BF16,
-                  ws.data_ptr() if n else None, n, st.data_ptr() if st is not None else None, c_stream(dev))
+    _call_on(dev, "vqmoe_grouped_linear", d, x.data_ptr(), P, _pitch(x),
+             offsets.data_ptr() if offsets is not None else None, out.data_ptr(),
+             _lib.OUT_F32 if out.dtype is torch.float32 else _lib.OUT_BF16,
+             ws.data_ptr() if n else None, n, st.data_ptr() if st is not None else None)
     return out
 
 
@@ -135,18 +147,18 @@ class Fp8Linear(nn.Module):
     def descriptor(self) -> _lib.Linear:
         w = self.weight
         require_cuda(w, self.weight_scale_inv)
-        return _lib.Linear(format=_lib.FMT_FP8_BLOCK, num_experts=1, out_features=w.shape[0], in_features=w.shape[1],
-                           weight=w.data_ptr(), scales=self.weight_scale_inv.data_ptr(), group_size=GROUP)
+        return fp8_descriptor(self, 1)
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        require_cuda(x)
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise TypeError(f"out_dtype {out_dtype} (bfloat16 or float32)")
-        _same_device(x, weight=self.weight)
-        xr = _rows(x, self.in_features)
-        out = torch.empty((*x.shape[:-1], self.out_features), dtype=out_dtype, device=x.device)
-        _run(self.descriptor(), xr, None, out)
-        return out
+        w = self._buffers["weight"]
+        N, K = w.shape
+        xr = _rows(x, K)
+        if w.device != x.device:
+            _same_device(x, weight=w)
+        out = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
+        return _run(fp8_descriptor(self, 1), xr, None, out)
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,

@@ -30,7 +30,10 @@ def _stream(t: torch.Tensor):
 
 
 def c_stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    i = device.index if isinstance(device, torch.device) else None
+    if i is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(i)
 
 
 def require_cuda(*ts: torch.Tensor) -> None:
@@ -370,6 +373,19 @@ def check_fp8_weight(weight: torch.Tensor, scales: torch.Tensor, dims: int) -> N
                          f"{tuple(weight.shape)} is {shape}")
 
 
+def fp8_descriptor(module: nn.Module, experts: int) -> _lib.Linear:
+    """The descriptor of a module's `weight` and `weight_scale_inv`, built
+    again when either lies elsewhere (the caller changes nothing in it)."""
+    w, s = module._buffers["weight"], module._buffers["weight_scale_inv"]
+    wp, sp = w.data_ptr(), s.data_ptr()
+    d = module.__dict__.get("_descriptor")
+    if d is None or d.weight != wp or d.scales != sp:
+        d = _lib.Linear(format=_lib.FMT_FP8_BLOCK, num_experts=experts, out_features=w.shape[-2],
+                        in_features=w.shape[-1], weight=wp, scales=sp, group_size=128)
+        module.__dict__["_descriptor"] = d
+    return d
+
+
 class Fp8SwitchLinear(_SwitchBase):
     """Block-scaled e4m3 experts, as block-quantized checkpoints store them:
     `weight [E, OUT, IN]` float8_e4m3fn and `weight_scale_inv [E,
@@ -401,9 +417,7 @@ class Fp8SwitchLinear(_SwitchBase):
 
     def descriptor(self) -> _lib.Linear:
         require_cuda(self.weight, self.weight_scale_inv)
-        return _lib.Linear(format=_lib.FMT_FP8_BLOCK, num_experts=self.num_experts,
-                           out_features=self.output_dims, in_features=self.input_dims,
-                           weight=self.weight.data_ptr(), scales=self.weight_scale_inv.data_ptr(), group_size=128)
+        return _lib.Linear.from_buffer_copy(fp8_descriptor(self, self.weight.shape[0]))
 
 
 class SwiGLU(nn.Module):

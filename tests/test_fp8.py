@@ -322,7 +322,9 @@ def grouped_64(x, w, off):
 GROUPED = [("uniform", 4, 1, 16, 16), ("uniform", 8, 40, 144, 272), ("skew", 16, 300, 272, 400),
            ("one", 5, 260, 128, 128), ("uniform", 128, 512, 256, 512), ("skew", 7, 900, 528, 336),
            ("uniform", 1, 129, 256, 144), ("uniform", 1024, 700, 16, 64), ("none", 6, 12, 32, 32),
-           ("one", 200, 17, 720, 1360), ("skew", 3, 1500, 400, 1040)]
+           ("one", 200, 17, 720, 1360), ("skew", 3, 1500, 400, 1040),
+           # several tiles a CTA, more scale blocks than accumulators
+           ("uniform", 128, 600, 768, 1168), ("skew", 100, 2000, 640, 2064)]
 
 
 @pytest.mark.gpu
@@ -426,7 +428,7 @@ def experts_64(x, idx, gate, up, down, kind="swiglu"):
 
 EXPERTS = [(1, 8, 2, 256, 128), (1, 64, 8, 2048, 768), (3, 16, 4, 272, 144), (24, 16, 4, 512, 256),
            (64, 64, 8, 640, 384), (300, 8, 2, 400, 272), (700, 4, 3, 256, 144), (2100, 8, 2, 128, 128),
-           (40, 200, 1, 144, 400)]
+           (40, 200, 1, 144, 400), (60, 128, 8, 1168, 384)]
 
 
 @pytest.mark.gpu
