@@ -13,8 +13,9 @@ What runs where on the GPU:
     experts, shared expert, combine);
   * every RMSNorm and the residual adds around it: `vqmoe_add_rms_norm`
     (libvqmoe), including the attention's per-head q/k norms;
-  * projections, embeddings and the LM head: cuBLAS through torch (plain
-    bf16 GEMMs); attention: torch's scaled-dot-product attention (a library
+  * projections and the LM head: cuBLAS through torch (plain bf16 GEMMs), or
+    `Fp8Linear` (libvqmoe) where the state dict holds them block-scaled
+    (`weight` float8_e4m3fn, `weight_scale_inv`); embeddings: torch; attention: torch's scaled-dot-product attention (a library
     kernel) over a per-sequence KV cache; rotary embedding: torch elementwise.
 The decoder follows the baseline's C5 description -- every layer full GQA
 attention (32 query / 4 key-value heads of 128) -- where the reference's
@@ -31,6 +32,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, synth
+from .fp8 import Fp8Linear
 from .moe import SparseMoeBlock
 from .switch_layers import c_stream, require_cuda
 
@@ -51,6 +53,7 @@ class DecoderConfig:
     partial_rotary: float = 0.25         # qwen3_5.py:237: rotary over a quarter of each head
     eps: float = 1e-6                    # qwen3_5.py:202
     mtp: bool = True                     # a one-layer MTP head
+    fp8: bool = False                    # random weights: projections and LM head block-scaled e4m3
 
     @property
     def rotary_dims(self) -> int:
@@ -88,13 +91,25 @@ def make_weights(cfg: DecoderConfig, seed: int = 0, device="cpu", scales: str = 
          "model.norm.weight": gain(H),
          "lm_head.weight": normal((cfg.vocab, H))}
 
+    def dense(name, shape):
+        """A projection: bf16, or block-scaled e4m3."""
+        if not cfg.fp8:
+            w[name + ".weight"] = normal(shape)
+            return
+        for leaf, t in synth._fp8_matrix(1, *shape, g, device).items():
+            w[f"{name}.{leaf}"] = t[0]
+
+    if cfg.fp8:
+        del w["lm_head.weight"]
+        dense("lm_head", (cfg.vocab, H))
+
     def layer(p, lseed):
         w[p + "input_layernorm.weight"] = gain(H)
         w[p + "post_attention_layernorm.weight"] = gain(H)
-        w[p + "self_attn.q_proj.weight"] = normal((nh * 2 * d, H))     # queries and the output gate
-        w[p + "self_attn.k_proj.weight"] = normal((kv * d, H))
-        w[p + "self_attn.v_proj.weight"] = normal((kv * d, H))
-        w[p + "self_attn.o_proj.weight"] = normal((H, nh * d))
+        dense(p + "self_attn.q_proj", (nh * 2 * d, H))                 # queries and the output gate
+        dense(p + "self_attn.k_proj", (kv * d, H))
+        dense(p + "self_attn.v_proj", (kv * d, H))
+        dense(p + "self_attn.o_proj", (H, nh * d))
         w[p + "self_attn.q_norm.weight"] = gain(d)
         w[p + "self_attn.k_norm.weight"] = gain(d)
         w.update(synth.make_weights(cfg.moe, seed=lseed, device=device, scales=scales, prefix=p + "mlp."))
@@ -133,6 +148,15 @@ def _gain(w: torch.Tensor) -> torch.Tensor:
 def _sigmoid_bf16(x: torch.Tensor) -> torch.Tensor:
     """`_sigmoid` (qwen3_5.py:35-36): in float32, rounded once."""
     return torch.sigmoid(x.float()).to(torch.bfloat16)
+
+
+def _linear(w: dict, name: str):
+    """The projection `{name}.weight` of a state dict as a function of x:
+    block-scaled e4m3 (`{name}.weight_scale_inv` beside it) or bf16."""
+    wt, sc = w[name + ".weight"], w.get(name + ".weight_scale_inv")
+    if sc is not None:
+        return Fp8Linear(wt, sc)
+    return lambda x: F.linear(x, wt)
 
 
 # --------------------------------------------------------------- attention
@@ -182,10 +206,7 @@ class Attention:
 
     def __init__(self, w: dict, p: str, cfg: DecoderConfig):
         self.cfg = cfg
-        self.wq = w[p + "q_proj.weight"]
-        self.wk = w[p + "k_proj.weight"]
-        self.wv = w[p + "v_proj.weight"]
-        self.wo = w[p + "o_proj.weight"]
+        self.wq, self.wk, self.wv, self.wo = (_linear(w, p + n) for n in ("q_proj", "k_proj", "v_proj", "o_proj"))
         self.q_norm = _gain(w[p + "q_norm.weight"])
         self.k_norm = _gain(w[p + "k_norm.weight"])
 
@@ -196,11 +217,11 @@ class Attention:
         c = self.cfg
         B, L, _ = x.shape
         nh, kv, d = c.heads, c.kv_heads, c.head_dim
-        q = F.linear(x, self.wq).view(B, L, nh, 2 * d)
+        q = self.wq(x).view(B, L, nh, 2 * d)
         queries = add_rms_norm(q[..., :d].contiguous(), None, self.q_norm, c.eps)
         gate = q[..., d:].reshape(B, L, nh * d)
-        keys = add_rms_norm(F.linear(x, self.wk).view(B, L, kv, d), None, self.k_norm, c.eps)
-        values = F.linear(x, self.wv).view(B, L, kv, d)
+        keys = add_rms_norm(self.wk(x).view(B, L, kv, d), None, self.k_norm, c.eps)
+        values = self.wv(x).view(B, L, kv, d)
         queries = rope(queries, pos0, c.rotary_dims, c.rope_theta)
         keys = rope(keys, pos0, c.rotary_dims, c.rope_theta)
         rep = nh // kv
@@ -213,7 +234,7 @@ class Attention:
             o = F.scaled_dot_product_attention(Q, cache.k.transpose(1, 2), cache.v.transpose(1, 2), attn_mask=mask,
                                                scale=d ** -0.5)
             o = o.view(B, kv, rep, L, d).permute(0, 3, 1, 2, 4).reshape(B, L, nh * d)
-            return F.linear(o * _sigmoid_bf16(gate), self.wo)
+            return self.wo(o * _sigmoid_bf16(gate))
         if pos0 + L > cache.max_len:
             raise ValueError(f"KV cache of {cache.max_len} positions: writing {pos0}..{pos0 + L}")
         cache.k[:, pos0:pos0 + L] = keys
@@ -237,7 +258,7 @@ class Attention:
                 o = F.scaled_dot_product_attention(Q, K, V, attn_mask=mask, scale=d ** -0.5)
             o = o.view(B, kv, rep, L, d).permute(0, 3, 1, 2, 4)
         o = o.reshape(B, L, nh * d)
-        return F.linear(o * _sigmoid_bf16(gate), self.wo)
+        return self.wo(o * _sigmoid_bf16(gate))
 
 
 class DecoderLayer:
@@ -290,6 +311,7 @@ class TextModel:
                 _release(self.layers[-1].mlp)
         self.norm = _gain(w["model.norm.weight"])
         self.lm_head = w["lm_head.weight"]
+        self.fp8_head = Fp8Linear(self.lm_head, w["lm_head.weight_scale_inv"]) if "lm_head.weight_scale_inv" in w else None
         self.mtp = MTPHead(w, cfg, self) if cfg.mtp else None
         if consume and self.mtp is not None:
             _drop(w, "mtp.layers.0.mlp.switch_mlp.")
@@ -314,7 +336,7 @@ class TextModel:
         return normed, pre
 
     def logits(self, normed: torch.Tensor) -> torch.Tensor:
-        return F.linear(normed, self.lm_head)
+        return F.linear(normed, self.lm_head) if self.fp8_head is None else self.fp8_head(normed)
 
 
 class MTPHead:
@@ -389,6 +411,8 @@ def _argmax(model: TextModel, normed: torch.Tensor) -> torch.Tensor:
     a tie would be broken by rounding noise that differs between a 1-wide
     and a (k+1)-wide forward."""
     H = normed.shape[-1]
+    if model.fp8_head is not None:
+        return model.fp8_head(normed, out_dtype=torch.float32).argmax(dim=-1)
     lg = torch.mm(normed.reshape(-1, H), model.lm_head.t(), out_dtype=torch.float32)
     return lg.argmax(dim=-1).view(normed.shape[:-1])
 

@@ -26,7 +26,7 @@ from torch import nn
 
 from . import _lib
 from .switch_layers import (Fp8SwitchLinear, QuantizedSwitchLinear, SwitchGLU, SwitchLinear, VQSwitchLinear, c_stream,
-                            require_cuda)
+                            check_fp8_weight, require_cuda)
 
 
 def _bf16_linear(weight: torch.Tensor) -> nn.Linear:
@@ -46,6 +46,20 @@ def tp_reduce(part: torch.Tensor, group) -> torch.Tensor:
         raise TypeError(f"partials must be float32, got {part.dtype}")
     dist.all_reduce(part, op=dist.ReduceOp.SUM, group=group)
     return part.to(torch.bfloat16)
+
+
+def dense_weight(w: dict, name: str) -> torch.Tensor:
+    """`{name}.weight` as a bf16 matmul takes it: a block-scaled e4m3 one
+    (`{name}.weight_scale_inv` beside it, a float32 for each 128 x 128 block)
+    restored to bf16, rounded once."""
+    wt, sc = w[name + ".weight"], w.get(name + ".weight_scale_inv")
+    if sc is None:
+        if wt.dtype == torch.float8_e4m3fn:
+            raise ValueError(f"{name}.weight is float8_e4m3fn without {name}.weight_scale_inv")
+        return wt
+    check_fp8_weight(wt, sc, 2)
+    full = sc.to(torch.float32).repeat_interleave(128, 0)[:wt.shape[0]].repeat_interleave(128, 1)[:, :wt.shape[1]]
+    return (wt.to(torch.float32) * full).to(torch.bfloat16)
 
 
 class SharedExpert(nn.Module):
@@ -238,13 +252,17 @@ class SparseMoeBlock(nn.Module):
         fused `{prefix}experts.gate_up_proj [E, 2I, H]` /
         `{prefix}experts.down_proj [E, H, I]` (split as
         `qwen3_5_moe.py:36-50`); `{prefix}shared_expert.{gate,up,down}_proj.`
-        `weight`, `{prefix}shared_expert_gate.weight`. `router_mode` and
+        `weight` (a block-scaled e4m3 one is restored to bf16),
+        `{prefix}shared_expert_gate.weight`. `router_mode` and
         `activation` (a `SwiGLU` or `GeGLU`) select the router and the
         experts' activation variants."""
         p = prefix
         sw = f"{p}switch_mlp."
         if f"{p}experts.gate_up_proj" in w:
             gu = w[f"{p}experts.gate_up_proj"]
+            if gu.dtype == torch.float8_e4m3fn:
+                raise ValueError(f"{p}experts.gate_up_proj is float8_e4m3fn: block-scaled experts are read from "
+                                 f"{sw}*_proj.weight and .weight_scale_inv")
             mid = gu.shape[-2] // 2
             projs = {"gate_proj": SwitchLinear(gu[..., :mid, :]),
                      "up_proj": SwitchLinear(gu[..., mid:, :]),
@@ -268,15 +286,15 @@ class SparseMoeBlock(nn.Module):
                 elif q + "weight_scale_inv" in w:
                     projs[n] = Fp8SwitchLinear(w[q + "weight"], w[q + "weight_scale_inv"])
                 elif q + "weight" in w:
+                    if w[q + "weight"].dtype == torch.float8_e4m3fn:
+                        raise KeyError(f"{q}weight is float8_e4m3fn: {q}weight_scale_inv is missing")
                     projs[n] = SwitchLinear(w[q + "weight"])
                 else:
                     raise KeyError(f"no weights for {q}")
         se = None
         seg = None
         if f"{p}shared_expert.gate_proj.weight" in w:
-            se = SharedExpert(w[f"{p}shared_expert.gate_proj.weight"],
-                              w[f"{p}shared_expert.up_proj.weight"],
-                              w[f"{p}shared_expert.down_proj.weight"])
+            se = SharedExpert(*(dense_weight(w, f"{p}shared_expert.{n}_proj") for n in ("gate", "up", "down")))
             seg = w[f"{p}shared_expert_gate.weight"]
         return cls(w[f"{p}gate.weight"], SwitchGLU(**projs, activation=activation), top_k, se, seg,
                    sharding_group=sharding_group, router_mode=router_mode, tp_reduce=tp_reduce,
