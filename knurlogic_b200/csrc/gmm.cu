@@ -287,7 +287,7 @@ enum Mode { kSingle = 0, kSplit = 1, kPair = 2, kSmall = 3 };
 constexpr int kAccCols = 256;                  // accumulator columns: two halves of 128
 constexpr int kThreads = 384;                  // TMA, MMA, two idle warps, eight epilogue warps
 constexpr int kCtlRegs = 40, kEpiRegs = 232;   // setmaxnreg: 128 x 40 + 256 x 232 = 384 x 168
-constexpr int kGroup = 4, kSlots = 3;          // scale blocks of a slot of staged scales, and the slots
+constexpr int kGroup = 4, kSlots = 3;          // scale blocks of a staged slot, and the slots
 constexpr int kMaxStages = 8;
 constexpr int kRingBytes = 160 * 1024;
 constexpr int kPartPitch = 257;                // floats of a row of partial sums (kSplit)
@@ -355,6 +355,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // staged products of token and weight scales: [slot][block][half, or gate / up][row]
     __shared__ float s_scale[FP8 ? kSlots * kGroup * 2 * kLanes : 1];
     __shared__ uint64_t sc_full[kSlots], sc_empty[kSlots];
+    // with a tile's first slot: the tile, its rows' output rows (-1: none) and their factors
+    __shared__ int4 s_tile[kSlots];
+    __shared__ int s_row[kSlots][kLanes];
+    __shared__ float s_rs[GLU ? 1 : kSlots][kLanes];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int bm = PAIR ? kLanes : p.bm, stages = p.stages;
@@ -515,40 +519,66 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-        else if (FP8 && warp >= 2) {
-            // ---- scales: warps 2 and 3 stage the products of the scales for
-            // the epilogue, a few blocks ahead of it. (Loaded by the epilogue
-            // itself, however far ahead, they cost it their latency in every
-            // block: 1240 cycles a block against 640.)
+        else if (warp >= 2) {
+            // ---- stagers: warps 2 and 3 find the tiles for the epilogue, a few
+            // blocks ahead of it, with their output rows and (e4m3) the products
+            // of the blocks' scales. (Loaded by the epilogue itself, however far
+            // ahead, the scales cost it their latency in every block: 1240
+            // cycles a block against 640.)
             const int l = tid - 64;                 // rows l and l + 64
-            const int NB = (a.N + kScaleBlock - 1) / kScaleBlock, units = kb1 - kb0;
+            const int NB = (a.N + kScaleBlock - 1) / kScaleBlock, units = FP8 ? kb1 - kb0 : 1;
             int slot = 0;
             uint32_t phase = 1;
             for (int tile = first; tile < tiles; tile += step) {
                 const Tile t = locate(a, s_g, tile, ntiles, tile_rows);
                 const int nb = GLU ? t.nt : 2 * t.nt;
-                const float *w0 = a.sw0 + ((size_t)t.e * NB + nb) * a.KB + kb0;
-                const float *w1 = GLU ? a.sw1 + ((size_t)t.e * NB + nb) * a.KB + kb0 : w0 + (nb + 1 < NB ? a.KB : 0);
-                const int r = t.row0 + (PAIR ? kLanes * rank : 0) + l;
-                const float *x0 = a.sx + (size_t)kb0 * a.P + min(r, a.P - 1), *x1 = x0 + min(64, a.P - 1 - min(r, a.P - 1));
+                const int r = t.row0 + (PAIR ? kLanes * rank : 0) + l, r1 = r + 64;
+                const bool live0 = l < bm && r < t.end, live1 = l + 64 < bm && r1 < t.end;
+                int o0 = live0 ? r : -1, o1 = live1 ? r1 : -1;
+                float rs0 = 1.0f, rs1 = 1.0f;
+                if (!GLU) {
+                    if (a.map && live0) o0 = __ldg(a.map + r);
+                    if (a.map && live1) o1 = __ldg(a.map + r1);
+                    if (a.row_scale && live0) rs0 = __ldg(a.row_scale + o0);
+                    if (a.row_scale && live1) rs1 = __ldg(a.row_scale + o1);
+                }
+                const float *w0 = nullptr, *w1 = nullptr, *x0 = nullptr, *x1 = nullptr;
+                if (FP8) {
+                    w0 = a.sw0 + ((size_t)t.e * NB + nb) * a.KB + kb0;
+                    w1 = GLU ? a.sw1 + ((size_t)t.e * NB + nb) * a.KB + kb0 : w0 + (nb + 1 < NB ? a.KB : 0);
+                    x0 = a.sx + (size_t)kb0 * a.P + min(r, a.P - 1);
+                    x1 = a.sx + (size_t)kb0 * a.P + min(r1, a.P - 1);
+                }
                 for (int i0 = 0; i0 < units; i0 += kGroup) {
                     float v[kGroup][4];
+                    if (FP8)
 #pragma unroll
-                    for (int z = 0; z < kGroup; ++z) {
-                        const int i = min(i0 + z, units - 1);
-                        v[z][0] = __ldg(x0 + (size_t)i * a.P);
-                        v[z][1] = __ldg(x1 + (size_t)i * a.P);
-                        v[z][2] = __ldg(w0 + i);
-                        v[z][3] = __ldg(w1 + i);
-                    }
+                        for (int z = 0; z < kGroup; ++z) {
+                            const int i = min(i0 + z, units - 1);
+                            v[z][0] = __ldg(x0 + (size_t)i * a.P);
+                            v[z][1] = __ldg(x1 + (size_t)i * a.P);
+                            v[z][2] = __ldg(w0 + i);
+                            v[z][3] = __ldg(w1 + i);
+                        }
                     wait(&sc_empty[slot], phase);
-                    float *to = s_scale + slot * kGroup * 2 * kLanes + l;
+                    if (FP8) {
+                        float *to = s_scale + slot * kGroup * 2 * kLanes + l;
 #pragma unroll
-                    for (int z = 0; z < kGroup; ++z, to += 2 * kLanes) {
-                        to[0] = v[z][0] * v[z][2];
-                        to[64] = v[z][1] * v[z][2];
-                        to[kLanes] = v[z][0] * v[z][3];
-                        to[kLanes + 64] = v[z][1] * v[z][3];
+                        for (int z = 0; z < kGroup; ++z, to += 2 * kLanes) {
+                            to[0] = v[z][0] * v[z][2];
+                            to[64] = v[z][1] * v[z][2];
+                            to[kLanes] = v[z][0] * v[z][3];
+                            to[kLanes + 64] = v[z][1] * v[z][3];
+                        }
+                    }
+                    if (i0 == 0) {
+                        if (l == 0) s_tile[slot] = make_int4(t.e, t.row0, t.end, t.nt);
+                        s_row[slot][l] = o0;
+                        s_row[slot][l + 64] = o1;
+                        if (!GLU) {
+                            s_rs[slot][l] = rs0;
+                            s_rs[slot][l + 64] = rs1;
+                        }
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sc_full[slot]);
@@ -578,21 +608,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         int slot = 0;
         bool ready = false;
         for (int tile = first; tile < tiles; tile += step) {
-            const Tile t = locate(a, s_g, tile, ntiles, tile_rows);
-            const int r = t.row0 + (PAIR ? kLanes * rank : 0) + row;
-            const bool live = row < bm && r < t.end;
-            const int n0 = t.nt * kOutCols + half * (kOutCols / 2);   // its first output column
+            Tile t{};
+            int orow = -1;                          // its output row
+            float rs = 1.0f;
             uint64_t acc[64];                       // 128 float32 sums
             if (FP8) {
 #pragma unroll
                 for (int j = 0; j < 64; ++j) acc[j] = 0;
             }
-            int orow = live ? r : -1;               // its output row
-            if (!GLU && !SPLIT && a.map && live) orow = ld_here(a.map + r);
             const int units = FP8 ? kb1 - kb0 : 1;
             for (int i0 = 0; i0 < units; i0 += kGroup) {
-                if (FP8) wait(&sc_full[slot], sphase);
-                const float *sc = s_scale + slot * kGroup * 2 * kLanes + row;
+                wait(&sc_full[slot], sphase);
+                if (i0 == 0) {
+                    const int4 f = s_tile[slot];
+                    t = Tile{f.x, f.y, f.z, f.w};
+                    orow = s_row[slot][row];
+                    if (!GLU) rs = s_rs[GLU ? 0 : slot][row];
+                }
+                const float *sc = s_scale + (FP8 ? slot * kGroup * 2 * kLanes + row : 0);
 #pragma unroll
                 for (int z = 0; z < kGroup; ++z) {
                     if (i0 + z >= units) break;
@@ -640,15 +673,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         add(3);
                     }
                 }
-                if (FP8) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sc_empty[slot]);
-                    if (++slot == kSlots) {
-                        slot = 0;
-                        sphase ^= 1;
-                    }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sc_empty[slot]);
+                if (++slot == kSlots) {
+                    slot = 0;
+                    sphase ^= 1;
                 }
             }
+            const int n0 = t.nt * kOutCols + half * (kOutCols / 2);   // its first output column
             if (SPLIT) {
                 // the ring is idle: this CTA's sums, [row][column], rows at
                 // a pitch of 257 so that lanes (rows) meet no bank twice and
@@ -689,10 +721,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     rows.put(c, w[0], w[1], w[2], w[3]);
                 }
-                rows.flush(a.q_out + n0, a.N, live ? r : -1, a.N - n0);
-                if (half == 0 && live) a.s_out[(size_t)t.nt * a.P + r] = qs.s;
+                rows.flush(a.q_out + n0, a.N, orow, a.N - n0);
+                if (half == 0 && orow >= 0) a.s_out[(size_t)t.nt * a.P + orow] = qs.s;
             } else {
-                const int o = orow;
                 const RowStore<8> rows{patch, lane};
                 if (a.out_f32) {
                     uint8_t *y = reinterpret_cast<uint8_t *>(static_cast<float *>(a.out) + n0);
@@ -703,10 +734,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint64_t x0 = acc[16 * h + 2 * c], x1 = acc[16 * h + 2 * c + 1];
                             rows.put(c, (uint32_t)x0, (uint32_t)(x0 >> 32), (uint32_t)x1, (uint32_t)(x1 >> 32));
                         }
-                        rows.flush(y + 128 * h, 4 * a.out_stride, o, 4 * (a.N - n0) - 128 * h);
+                        rows.flush(y + 128 * h, 4 * a.out_stride, orow, 4 * (a.N - n0) - 128 * h);
                     }
                 } else {
-                    const float rs = a.row_scale && o >= 0 ? a.row_scale[o] : 1.0f;
                     uint8_t *y = reinterpret_cast<uint8_t *>(static_cast<uint16_t *>(a.out) + n0);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -721,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                             rows.put(c, w[0], w[1], w[2], w[3]);
                         }
-                        rows.flush(y + 128 * h, 2 * a.out_stride, o, 2 * (a.N - n0) - 128 * h);
+                        rows.flush(y + 128 * h, 2 * a.out_stride, orow, 2 * (a.N - n0) - 128 * h);
                     }
                 }
             }
