@@ -18,8 +18,8 @@
 // token scale is one register) x 256 weight rows (gate/up: 128 of each), with
 // two TMEM buffers. Persistent CTAs of specialised warps: warp 0 issues TMA
 // copies of 128-byte rows into a ring of 128-byte-swizzled stages, warp 1
-// issues the MMAs, warps 4-7 and 8-11 are the epilogues of the accumulator's
-// two halves of 128 columns. Three modes:
+// issues the MMAs, warps 2 and 3 stage what the epilogue reads, and sixteen
+// warps are the epilogue, 64 accumulator columns each. Three modes:
 //   kPair    two CTAs (cta_group::2) share a tile of 256 tokens: each loads its
 //            128 tokens and half of the weight rows, so a block costs a CTA 32
 //            KB of L2 reads instead of 48. Many tokens a group.
@@ -164,6 +164,16 @@ __device__ __forceinline__ int ld_here(const int *p) {   // not sunk to its use
     return v;
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+        "%13, %14, %15}, [%16];\n"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 // One lane of the (converged) warp. The roles that issue copies and MMAs run
 // their loops with the whole warp and elect a lane for the issue alone: the
 // loop stays uniform, so descriptors and barriers are built in uniform
@@ -285,14 +295,15 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
 enum Mode { kSingle = 0, kSplit = 1, kPair = 2, kSmall = 3 };
 
 constexpr int kAccCols = 256;                  // accumulator columns: two halves of 128
-constexpr int kThreads = 384;                  // TMA, MMA, two idle warps, eight epilogue warps
-constexpr int kCtlRegs = 40, kEpiRegs = 232;   // setmaxnreg: 128 x 40 + 256 x 232 = 384 x 168
+constexpr int kEpiWarps = 16;                  // a warp of the accumulator's 32 lanes takes 64 columns
+constexpr int kThreads = 32 * (4 + kEpiWarps); // TMA, MMA, two stagers, the epilogue
+constexpr int kCtlRegs = 56, kEpiRegs = 104;   // setmaxnreg: 128 x 56 + 512 x 104 of the 640 x 96 at launch
 constexpr int kGroup = 4, kSlots = 3;          // scale blocks of a staged slot, and the slots
 constexpr int kMaxStages = 8;
 constexpr int kRingBytes = 160 * 1024;
 constexpr int kPartPitch = 257;                // floats of a row of partial sums (kSplit)
-constexpr int kPatch = 4096;                   // an epilogue warp's output staging: 32 rows of 128 bytes
-constexpr size_t kSmem = 1024 + kRingBytes + 8 * kPatch;
+constexpr int kPatch = 2048;                   // an epilogue warp's output staging: 32 rows of 64 bytes
+constexpr size_t kSmem = 1024 + kRingBytes + kEpiWarps * kPatch;
 
 // SwiGLU / GeGLU of two columns, every step rounded to bf16: packed bf16
 __device__ __forceinline__ uint32_t glu_pair(float g0, float g1, float u0, float u1, int act) {
@@ -320,7 +331,7 @@ struct RowStore {
     uint8_t *patch;
     int lane;
     __device__ static int at(int row, int c) {
-        return row * (CH * 16) + 16 * (c ^ (CH == 8 ? row & 7 : (row >> 1) & 3));
+        return row * (CH * 16) + 16 * (c ^ (CH == 4 ? (row >> 1) & 3 : (row >> 2) & 1));
     }
     __device__ void put(int c, uint32_t a, uint32_t b, uint32_t d, uint32_t e) const {
         *reinterpret_cast<uint4 *>(patch + at(lane, c)) = make_uint4(a, b, d, e);
@@ -351,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t s_tmem;
     __shared__ Groups s_g;
-    __shared__ uint32_t s_amax[GLU ? 2 * kLanes : 1];
+    __shared__ uint32_t s_amax[GLU ? 4 * kLanes : 1];
     // staged products of token and weight scales: [slot][block][half, or gate / up][row]
     __shared__ float s_scale[FP8 ? kSlots * kGroup * 2 * kLanes : 1];
     __shared__ uint64_t sc_full[kSlots], sc_empty[kSlots];
@@ -374,11 +385,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], PAIR ? 16 : 8);
+            mbar_init(&acc_empty[i], (PAIR ? 2 : 1) * kEpiWarps);
         }
         for (int i = 0; i < kSlots; ++i) {
             mbar_init(&sc_full[i], 2);
-            mbar_init(&sc_empty[i], 8);
+            mbar_init(&sc_empty[i], kEpiWarps);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -595,13 +606,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             cluster_arrive_wait();
         }
     } else {
-        // ---- epilogue: thread = one token, one half of the tile's columns:
-        // 128 weight rows, or (gate/up) 64 of each matrix
+        // ---- epilogue: thread = one token, a quarter of the tile's columns:
+        // 64 weight rows, or (gate/up) 32 of each matrix
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kEpiRegs));
-        const int q = warp & 3, half = (warp - 4) >> 2, row = 32 * q + lane;
+        const int q = warp & 3, part = (warp - 4) >> 2, half = part >> 1, row = 32 * q + lane;
         const bool busy = 32 * q < bm;              // lanes that hold token rows at all
         uint8_t *const patch = smem_raw + (sbase - smem_u32(smem_raw)) + kRingBytes + (warp - 4) * kPatch;
-        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16) + half * 128;
+        // its accumulator columns: two pieces of 32
+        const int col0 = GLU ? 128 * half + 32 * (part & 1) : 64 * part, col1 = col0 + (GLU ? 64 : 32);
+        const uint32_t tq = tmem + ((uint32_t)(32 * q) << 16);
         // the accumulators' barriers for the MMA issuer, a pair's in its leader
         const uint32_t done0 = map_cluster(smem_u32(&acc_empty[0]), 0);
         uint32_t un = 0, sphase = 0;
@@ -611,10 +624,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             Tile t{};
             int orow = -1;                          // its output row
             float rs = 1.0f;
-            uint64_t acc[64];                       // 128 float32 sums
+            uint64_t acc[32];                       // 64 float32 sums
             if (FP8) {
 #pragma unroll
-                for (int j = 0; j < 64; ++j) acc[j] = 0;
+                for (int j = 0; j < 32; ++j) acc[j] = 0;
             }
             const int units = FP8 ? kb1 - kb0 : 1;
             for (int i0 = 0; i0 < units; i0 += kGroup) {
@@ -626,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!GLU) rs = s_rs[GLU ? 0 : slot][row];
                 }
                 const float *sc = s_scale + (FP8 ? slot * kGroup * 2 * kLanes + row : 0);
-#pragma unroll
+#pragma unroll 1
                 for (int z = 0; z < kGroup; ++z) {
                     if (i0 + z >= units) break;
                     uint64_t s0 = 0, s1 = 0;
@@ -642,24 +655,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                     wait(&acc_full[u], (un >> 1) & 1, ready);
                     ++un;
                     tc_fence_after();
-                    uint32_t dv[2][32];
+                    uint32_t dv[16];
                     auto add = [&](int c) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const uint64_t v = pack2(dv[c & 1][2 * j], dv[c & 1][2 * j + 1]);
-                            if (FP8) fma2(acc[16 * c + j], v, c < 2 ? s0 : s1);
-                            else acc[16 * c + j] = v;
+                        for (int j = 0; j < 8; ++j) {
+                            const uint64_t v = pack2(dv[2 * j], dv[2 * j + 1]);
+                            if (FP8) fma2(acc[8 * c + j], v, c >= 2 ? s1 : s0);
+                            else acc[8 * c + j] = v;
                         }
                     };
                     if (busy) {
-                        tmem_ld32(td, dv[0]);
-                        tmem_ld32(td + 32, dv[1]);
-                        tmem_wait_ld();
-                        add(0);
-                        tmem_ld32(td + 64, dv[0]);
-                        add(1);
-                        tmem_ld32(td + 96, dv[1]);
-                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            tmem_ld16(td + (c >= 2 ? col1 : col0) + 16 * (c & 1), dv);
+                            tmem_wait_ld();
+                            if (c < 3) add(c);
+                        }
                     }
                     // (every lane's tcgen05.ld is done: the wait is the warp's)
                     tc_fence_before();
@@ -668,10 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         else mbar_arrive(&acc_empty[u]);
                     }
                     ready = test_bar(&acc_full[un & 1], (un >> 1) & 1);
-                    if (busy) {
-                        add(2);
-                        add(3);
-                    }
+                    if (busy) add(3);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sc_empty[slot]);
@@ -680,38 +688,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sphase ^= 1;
                 }
             }
-            const int n0 = t.nt * kOutCols + half * (kOutCols / 2);   // its first output column
+            const int n0 = t.nt * kOutCols + part * (kOutCols / 4);   // its first output column
             if (SPLIT) {
                 // the ring is idle: this CTA's sums, [row][column], rows at
                 // a pitch of 257 so that lanes (rows) meet no bank twice and
                 // the others read a row's columns in whole lines
-                float *part = reinterpret_cast<float *>(smem_raw + (sbase - smem_u32(smem_raw)));
+                float *sums = reinterpret_cast<float *>(smem_raw + (sbase - smem_u32(smem_raw)));
                 if (row < bm) {
-                    float *to = part + row * kPartPitch + half * 128;
+                    float *to = sums + row * kPartPitch;
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) {
-                        to[2 * j] = lo2(acc[j]);
-                        to[2 * j + 1] = hi2(acc[j]);
+                    for (int j = 0; j < 32; ++j) {
+                        const int c = (j < 16 ? col0 : col1 - 32) + 2 * j;
+                        to[c] = lo2(acc[j]);
+                        to[c + 1] = hi2(acc[j]);
                     }
                 }
             } else if (GLU) {
-                // 64 activations of the token's group of 128; the largest of
-                // all 128 with the other half's warp
-                uint32_t m = 0, v[32];
+                // 32 activations of the token's group of 128; the largest of
+                // all 128 with the other three warps of these lanes
+                uint32_t m = 0, v[16];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    v[j] = glu_pair(lo2(acc[j]), hi2(acc[j]), lo2(acc[32 + j]), hi2(acc[32 + j]), a.act);
+                for (int j = 0; j < 16; ++j) {
+                    v[j] = glu_pair(lo2(acc[j]), hi2(acc[j]), lo2(acc[16 + j]), hi2(acc[16 + j]), a.act);
                     if (n0 + 2 * j < a.N) m = __vmaxu2(m, v[j] & 0x7FFF7FFFu);
                 }
-                m = max(m & 0xFFFFu, m >> 16);
-                s_amax[half * kLanes + row] = m;
-                bar_sync(1, 256);
-                m = max(m, s_amax[(half ^ 1) * kLanes + row]);
-                bar_sync(1, 256);                   // read before the next tile's
+                s_amax[part * kLanes + row] = max(m & 0xFFFFu, m >> 16);
+                bar_sync(1, 32 * kEpiWarps);
+                m = max(max(s_amax[row], s_amax[kLanes + row]), max(s_amax[2 * kLanes + row], s_amax[3 * kLanes + row]));
+                bar_sync(1, 32 * kEpiWarps);        // read before the next tile's
                 const QScale qs = qscale(m);
-                const RowStore<4> rows{patch, lane};
+                const RowStore<2> rows{patch, lane};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 2; ++c) {
                     uint32_t w[4];
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
@@ -722,36 +730,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                     rows.put(c, w[0], w[1], w[2], w[3]);
                 }
                 rows.flush(a.q_out + n0, a.N, orow, a.N - n0);
-                if (half == 0 && orow >= 0) a.s_out[(size_t)t.nt * a.P + orow] = qs.s;
+                if (part == 0 && orow >= 0) a.s_out[(size_t)t.nt * a.P + orow] = qs.s;
             } else {
-                const RowStore<8> rows{patch, lane};
+                const RowStore<4> rows{patch, lane};
                 if (a.out_f32) {
                     uint8_t *y = reinterpret_cast<uint8_t *>(static_cast<float *>(a.out) + n0);
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const uint64_t x0 = acc[16 * h + 2 * c], x1 = acc[16 * h + 2 * c + 1];
+                        for (int c = 0; c < 4; ++c) {
+                            const uint64_t x0 = acc[8 * h + 2 * c], x1 = acc[8 * h + 2 * c + 1];
                             rows.put(c, (uint32_t)x0, (uint32_t)(x0 >> 32), (uint32_t)x1, (uint32_t)(x1 >> 32));
                         }
-                        rows.flush(y + 128 * h, 4 * a.out_stride, orow, 4 * (a.N - n0) - 128 * h);
+                        rows.flush(y + 64 * h, 4 * a.out_stride, orow, 4 * (a.N - n0) - 64 * h);
                     }
                 } else {
                     uint8_t *y = reinterpret_cast<uint8_t *>(static_cast<uint16_t *>(a.out) + n0);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
+                        for (int c = 0; c < 4; ++c) {
                             uint32_t w[4];
 #pragma unroll
                             for (int z = 0; z < 4; ++z) {
-                                const uint64_t x = acc[32 * h + 4 * c + z];
+                                const uint64_t x = acc[16 * h + 4 * c + z];
                                 w[z] = cvt_bf16x2(lo2(x), hi2(x));
                                 if (a.row_scale) w[z] = cvt_bf16x2(bf_lo(w[z]) * rs, bf_hi(w[z]) * rs);
                             }
                             rows.put(c, w[0], w[1], w[2], w[3]);
                         }
-                        rows.flush(y + 128 * h, 2 * a.out_stride, orow, 2 * (a.N - n0) - 128 * h);
+                        rows.flush(y + 64 * h, 2 * a.out_stride, orow, 2 * (a.N - n0) - 64 * h);
                     }
                 }
             }
@@ -765,35 +773,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Tile t = locate(a, s_g, first, ntiles, tile_rows);
                 const int np = min(bm, t.end - t.row0);
                 uint32_t peer[8];
-    #pragma unroll
+#pragma unroll
                 for (int c = 0; c < 8; ++c) peer[c] = map_cluster(sbase, min(c, S - 1));
                 // the cluster's sums of N (row, column)s, every load in flight
                 // before the first is used
                 auto sums = [&](auto &v, const auto &at) {
                     constexpr int N = sizeof(v) / sizeof(float);
                     float x[N][8];
-    #pragma unroll
+#pragma unroll
                     for (int c = 0; c < 8; ++c)
                         if (c < S)
-    #pragma unroll
+#pragma unroll
                             for (int n = 0; n < N; ++n) x[n][c] = ld_cluster(peer[c] + 4 * at(n));
-    #pragma unroll
+#pragma unroll
                     for (int n = 0; n < N; ++n) v[n] = 0.0f;
-    #pragma unroll
+#pragma unroll
                     for (int c = 0; c < 8; ++c)
                         if (c < S)
-    #pragma unroll
+#pragma unroll
                             for (int n = 0; n < N; ++n) v[n] += x[n][c];
                 };
                 if (GLU) {
-                    for (int u = (warp - 4) * S + rank; u < np; u += 8 * S) {
+                    for (int u = (warp - 4) * S + rank; u < np; u += kEpiWarps * S) {
                         float g[8], v[4];            // gate and up of this lane's four columns
                         uint32_t m = 0;
                         sums(g, [&](int n) {
                             const int c = lane + 32 * (n & 3);
                             return u * kPartPitch + (c >> 6) * 128 + (c & 63) + 64 * (n >> 2);
                         });
-    #pragma unroll
+#pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint32_t y = glu_pair(g[i], 0.0f, g[4 + i], 0.0f, a.act);
                             v[i] = bf_lo(y);
@@ -801,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         const QScale qs = qscale(__reduce_max_sync(0xffffffffu, m));
                         const size_t r = (size_t)(t.row0 + u);
-    #pragma unroll
+#pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int n = t.nt * 128 + lane + 32 * i;
                             if (n < a.N) a.q_out[r * a.N + n] = (uint8_t)cvt_e4m3x2(quotient(v[i], qs), 0.0f);
@@ -811,16 +819,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else {
                     // 32 columns of a row a warp and step, four steps at a time
                     constexpr int kSteps = 4;
-                    const int step8 = 8 * S, total = 8 * np;
-                    for (int u0 = (warp - 4) * S + rank; u0 < total; u0 += kSteps * step8) {
+                    const int stride = kEpiWarps * S, total = 8 * np;
+                    for (int u0 = (warp - 4) * S + rank; u0 < total; u0 += kSteps * stride) {
                         float v[kSteps];
                         sums(v, [&](int n) {
-                            const int u = min(u0 + n * step8, total - 1);
+                            const int u = min(u0 + n * stride, total - 1);
                             return (u >> 3) * kPartPitch + (u & 7) * 32 + lane;
                         });
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < kSteps; ++k) {
-                            const int u = u0 + k * step8, n = t.nt * 256 + (u & 7) * 32 + lane;
+                            const int u = u0 + k * stride, n = t.nt * 256 + (u & 7) * 32 + lane;
                             if (u >= total || n >= a.N) continue;
                             const int r = t.row0 + (u >> 3), o = a.map ? a.map[r] : r;
                             if (a.out_f32) {
@@ -864,11 +872,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kTok = 32;
 constexpr int kUnits = 4;                      // accumulators of a warpgroup
 constexpr int kSmallSlots = 2;                 // slots of staged scales of a warpgroup
+constexpr int kSmallThreads = 384;
 constexpr int kSmallRing = 184 * 1024;
 constexpr size_t kSmallSmem = 1024 + kSmallRing;
 
 template <int NMAT, bool FP8>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kSmallThreads, 1)
     gmm_small_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw0,
                      const __grid_constant__ CUtensorMap tw1, const GmmArgs a, const Plan p) {
     constexpr bool GLU = NMAT == 2;
@@ -1146,7 +1155,7 @@ static vqmoe_status check_registers(const void *fn) {
         if (cudaFuncGetAttributes(&at, fn) != cudaSuccess) return check_launch("gmm_kernel");
         n = at.numRegs;
     }
-    if (n * kThreads < 128 * kCtlRegs + 256 * kEpiRegs)
+    if (n * kThreads < 128 * kCtlRegs + 32 * kEpiWarps * kEpiRegs)
         return set_error(VQMOE_LAUNCH_FAILED, "gmm_kernel: built with %d registers a thread", n);
     return VQMOE_OK;
 }
@@ -1291,7 +1300,7 @@ vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const voi
         return s;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(mode == kSmall ? kSmallThreads : kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
