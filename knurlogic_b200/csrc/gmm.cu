@@ -32,6 +32,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <map>
 #include <mutex>
 
@@ -1169,13 +1170,10 @@ static bool byte_map(CUtensorMap *m, const void *base, size_t rows, size_t row_b
 // How many clusters of `size` CTAs of the kernel run at a time (each CTA takes
 // an SM, and a cluster stays inside one GPC), looked up once per device.
 static int max_clusters(const void *fn, int size) {
-    static std::mutex mu;
-    static std::map<std::pair<int, int>, int> known;
+    static std::atomic<int> known[64][9];          // the number + 1
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    std::lock_guard<std::mutex> lock(mu);
-    auto it = known.find({dev, size});
-    if (it != known.end()) return it->second;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (const int n = known[dev][size].load(std::memory_order_relaxed)) return n - 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(size);
     cfg.blockDim = dim3(kThreads);
@@ -1192,7 +1190,7 @@ static int max_clusters(const void *fn, int size) {
         cudaGetLastError();
         n = 0;
     }
-    known[{dev, size}] = n;
+    known[dev][size].store(n + 1, std::memory_order_relaxed);
     return n;
 }
 
@@ -1336,11 +1334,22 @@ __global__ void __launch_bounds__(256)
     const uint32_t slots = gridDim.x * 32, slot = blockIdx.x * 32 + (threadIdx.x >> 3);
     // every lane of a warp makes the same trips (the shuffles need all of them)
     const uint32_t trips = (total + slots - 1) / slots;
+    const int k = ORDER && !o.per_pair ? o.k : 1;
+    // the places of pairs y0 .. y0 + 7 of a row (-1: no such expert, no place)
+    auto places = [&](int (&at)[8], uint32_t row, int y0) {
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const size_t p = (size_t)row * k + min(y0 + y, k - 1);
+            const int rk = __ldg(o.rank + p), e = __ldg(o.inds + p);
+            at[y] = y0 + y < k && rk >= 0 ? __ldg(o.off + e) + rk : -1;
+        }
+    };
     for (uint32_t i0 = 0; i0 < trips; i0 += kQuantAhead) {
         uint4 v[kQuantAhead][2];
         uint32_t row[kQuantAhead];
         int c[kQuantAhead];
         bool in[kQuantAhead];
+        int at[ORDER ? kQuantAhead : 1][8];
 #pragma unroll
         for (int z = 0; z < kQuantAhead; ++z) {
             const uint32_t g = slot + (i0 + z) * slots;
@@ -1353,6 +1362,7 @@ __global__ void __launch_bounds__(256)
                 v[z][0] = __ldcs(p);
                 v[z][1] = __ldcs(p + 1);
             }
+            if (ORDER && in[z]) places(at[ORDER ? z : 0], row[z], 0);   // beside the values' own load
         }
 #pragma unroll
         for (int z = 0; z < kQuantAhead; ++z) {
@@ -1377,23 +1387,14 @@ __global__ void __launch_bounds__(256)
                 if (live) *reinterpret_cast<uint4 *>(q + (size_t)row[z] * cols + c[z]) = r;
                 if (lane == 0) s[row[z] * s_row + grp * s_group] = qs.s;
             } else {
-                // the places of the row's pairs, eight looked up at a time
-                const int k = o.per_pair ? 1 : o.k;
                 for (int y0 = 0; y0 < k; y0 += 8) {
-                    int rk[8], at[8];
+                    int (&to)[8] = at[ORDER ? z : 0];
+                    if (y0) places(to, row[z], y0);
 #pragma unroll
                     for (int y = 0; y < 8; ++y) {
-                        const size_t p = (size_t)row[z] * k + min(y0 + y, k - 1);
-                        rk[y] = y0 + y < k ? __ldg(o.rank + p) : -1;      // < 0: no such expert, no place
-                        at[y] = rk[y] >= 0 ? __ldg(o.inds + p) : 0;
-                    }
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) at[y] = rk[y] >= 0 ? __ldg(o.off + at[y]) + rk[y] : -1;
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        if (at[y] < 0) continue;
-                        if (live) *reinterpret_cast<uint4 *>(q + (size_t)at[y] * cols + c[z]) = r;
-                        if (lane == 0) s[at[y] * s_row + grp * s_group] = qs.s;
+                        if (to[y] < 0) continue;
+                        if (live) *reinterpret_cast<uint4 *>(q + (size_t)to[y] * cols + c[z]) = r;
+                        if (lane == 0) s[to[y] * s_row + grp * s_group] = qs.s;
                     }
                 }
             }

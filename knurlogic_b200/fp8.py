@@ -89,8 +89,9 @@ def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if K <= 0 or K % 16:
         raise ValueError(f"x {tuple(x.shape)}: the last dimension must be a multiple of 16")
     xr = _rows(x, K)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    s = torch.empty((*x.shape[:-1], -(-K // GROUP)), dtype=torch.float32, device=x.device)
+    q = (torch.empty_like(x, dtype=torch.float8_e4m3fn) if x.is_contiguous()
+         else x.new_empty(x.shape, dtype=torch.float8_e4m3fn))
+    s = x.new_empty((*x.shape[:-1], -(-K // GROUP)), dtype=torch.float32)
     if xr.shape[0]:
         _call_on(x.device, "vqmoe_quantize_fp8", xr.data_ptr(), xr.shape[0], K, _pitch(xr), q.data_ptr(), s.data_ptr())
     return q, s
@@ -103,7 +104,7 @@ def _run(d: _lib.Linear, x: torch.Tensor, offsets, out: torch.Tensor) -> torch.T
         return out
     dev = x.device
     n = _lib.lib().vqmoe_grouped_linear_workspace_size(d, P)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    ws = x.new_empty(n, dtype=torch.uint8) if n else None
     st = _status.get(dev.index)
     if st is None:
         st = _status_word(dev)
@@ -157,7 +158,7 @@ class Fp8Linear(nn.Module):
         xr = _rows(x, K)
         if w.device != x.device:
             _same_device(x, weight=w)
-        out = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=x.device)
+        out = x.new_empty((*x.shape[:-1], N), dtype=out_dtype)
         return _run(fp8_descriptor(self, 1), xr, None, out)
 
 
@@ -194,7 +195,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     if out is None:
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise TypeError(f"out_dtype {out_dtype} (bfloat16 or float32)")
-        out = torch.empty((x.shape[0], N), dtype=out_dtype, device=x.device)
+        out = x.new_empty((x.shape[0], N), dtype=out_dtype)
     elif (tuple(out.shape) != (x.shape[0], N) or out.dtype not in (torch.bfloat16, torch.float32)
           or not out.is_contiguous()):
         raise ValueError(f"out must be contiguous [{x.shape[0]}, {N}] bfloat16 or float32, got {tuple(out.shape)} "
