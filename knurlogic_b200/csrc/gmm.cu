@@ -326,7 +326,8 @@ struct Plan {
 // a store instruction writes whole rows: lane `lane` puts CH 16-byte chunks of
 // its row (put), and CH lanes then write each row (flush). A thread storing its
 // own row, 16 bytes in each of 32 rows an instruction, took 12800 cycles of a
-// 128 x 256 tile; this takes 1400.
+// 128 x 256 tile, and the tensor core waits for most of them; this takes 2300
+// to 3400.
 template <int CH>
 struct RowStore {
     uint8_t *patch;
@@ -534,9 +535,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         else if (warp >= 2) {
             // ---- stagers: warps 2 and 3 find the tiles for the epilogue, a few
             // blocks ahead of it, with their output rows and (e4m3) the products
-            // of the blocks' scales. (Loaded by the epilogue itself, however far
-            // ahead, the scales cost it their latency in every block: 1240
-            // cycles a block against 640.)
+            // of the blocks' scales. (With the tiles found and the output rows
+            // looked up by the epilogue a tile of six blocks took 11200 cycles,
+            // so 10400. The scales' loads in the epilogue's own loop would take
+            // a dozen of its registers and, with six scoreboards a warp, make
+            // it wait for the youngest.)
             const int l = tid - 64;                 // rows l and l + 64
             const int NB = (a.N + kScaleBlock - 1) / kScaleBlock, units = FP8 ? kb1 - kb0 : 1;
             int slot = 0;
@@ -1240,13 +1243,14 @@ vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const voi
     if (a.off) {
         // Ragged: the host knows the mean alone, so the tile goes by that.
         // Measured at 128 groups of 768 x 2048 (us; kSmall / kSingle with 64 /
-        // with 128 rows / kPair), even and Zipf-distributed groups: mean 4
-        // e4m3 42 / 46 / 48 / 69 and 37 / 45 / 46 / 58, bf16 70 / 68 / 71 / 86
-        // and 58 / 65 / 69 / 68; mean 16 e4m3 47 / 50 / 52 and 50 / 50 / 51,
-        // bf16 73 / 71 / 74 and 80 / 70 / 73; mean 32 e4m3 56 / 53 / 55 and 63 /
-        // 63 / 53; mean 256 (128 rows / kPair) e4m3 132 / 134, bf16 147 / 136;
-        // mean 512 e4m3 229 / 228, bf16 241 / 210. e4m3 gate/up and down: mean
-        // 32 150 / 190 / 196, mean 64 219 / 238 / 207, mean 512 692 / 709.
+        // with 128 rows / kPair), even groups, then Zipf-distributed ones: mean
+        // 4 e4m3 42 / 43 / 44 / 66, 36 / 34 / 35 / 47, bf16 69 / 69 / 73 / 82,
+        // 57 / 55 / 56 / 58; mean 16 e4m3 46 / 47 / 48 / 69, 51 / 46 / 48 / 71,
+        // bf16 72 / 72 / 75 / 86, 80 / 71 / 74 / 84; mean 32 e4m3 58 / 51 / 51 /
+        // 72, 65 / 60 / 51 / 73; mean 256 (128 rows / kPair) e4m3 136 / 141, 146 /
+        // 147, bf16 146 / 126, 149 / 135; mean 512 e4m3 247 / 232, bf16 235 / 192.
+        // e4m3 gate/up with down: mean 4 124 / 143 / 148 / 203, mean 32 156 / 156 /
+        // 162 (gate/up by kSmall, down by 128 rows: 148), mean 48 188 / 167 / 166.
         const int mean = (a.P + groups - 1) / groups;
         if (mean <= (glu ? 40 : fp8 ? 20 : 6)) consider(kSmall, kTok, 1, glu ? 0.74 : 0.37, 0.7, sms);
         else if (mean <= 24) consider(kSingle, 64, 1, 0.55, 3.0, sms);

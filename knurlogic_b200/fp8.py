@@ -19,7 +19,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .switch_layers import _contig, c_stream, check_fp8_weight, fp8_descriptor, require_cuda
+from .switch_layers import Fp8Buffers, _contig, c_stream, check_fp8_weight, fp8_descriptor, require_cuda
 
 GROUP = 128
 _status: dict = {}
@@ -121,7 +121,7 @@ def _same_device(x: torch.Tensor, **others: torch.Tensor) -> None:
             raise ValueError(f"{name} is on {t.device}, x on {x.device}")
 
 
-class Fp8Linear(nn.Module):
+class Fp8Linear(Fp8Buffers, nn.Module):
     """y = x W^T with block-scaled e4m3 weights: `weight [OUT, IN]`
     float8_e4m3fn, `weight_scale_inv [ceil(OUT/128), ceil(IN/128)]` (float32,
     or bf16 widened). OUT and IN are multiples of 16.

@@ -386,7 +386,17 @@ def fp8_descriptor(module: nn.Module, experts: int) -> _lib.Linear:
     return d
 
 
-class Fp8SwitchLinear(_SwitchBase):
+class Fp8Buffers:
+    """Modules with an `fp8_descriptor`: it holds addresses, so copies and
+    pickles leave it out."""
+
+    def __getstate__(self):
+        d = self.__dict__.copy()
+        d.pop("_descriptor", None)
+        return d
+
+
+class Fp8SwitchLinear(Fp8Buffers, _SwitchBase):
     """Block-scaled e4m3 experts, as block-quantized checkpoints store them:
     `weight [E, OUT, IN]` float8_e4m3fn and `weight_scale_inv [E,
     ceil(OUT/128), ceil(IN/128)]` float32 (the factor that restores a block;

@@ -11,6 +11,8 @@ bf16, none more for float32). With S the sum of the terms' magnitudes and K
 terms that is |got - ref| <= half * |ref| + (K + 4) 2^-23 S.
 Quantization is exact: its values and scales are compared bit for bit.
 """
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -263,6 +265,40 @@ def test_linear_shapes_strides_and_streams():
         m(big.float()[:, :272])
     with pytest.raises(ValueError, match="features"):
         m(big)
+
+
+@pytest.mark.gpu
+def test_a_copied_module_has_its_own_weights():
+    w, s = make_weight((144, 272), 5, DEV)
+    m, x = Fp8Linear(w, s), make_x(3, 272, 1, DEV)
+    y = m(x)
+    c = copy.deepcopy(m)
+    m.weight.view(torch.uint8).zero_()
+    assert torch.equal(c(x), y) and not m(x).any()
+    e = Fp8SwitchLinear(w[None].clone(), s[None])
+    e.descriptor()
+    assert "_descriptor" in e.__dict__ and "_descriptor" not in copy.deepcopy(e).__dict__
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_do_not_meet():
+    """Workspaces are each call's own: products and experts interleaved on
+    two streams give what they give alone."""
+    m = Fp8Linear(*make_weight((528, 1040), 5, DEV))
+    glu = SwitchGLU(*(Fp8SwitchLinear(*make_weight(sh, i, DEV)) for i, sh in
+                      enumerate([(8, 256, 1040), (8, 256, 1040), (8, 1040, 256)])))
+    xs = [make_x(T, 1040, T, DEV) for T in (3, 40, 300, 700)]
+    idx = [torch.randint(0, 8, (x.shape[0], 2), device=DEV, dtype=torch.int32) for x in xs]
+    alone = [(m(x), glu(x, i)) for x, i in zip(xs, idx)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(4):
+        for j, (x, i) in enumerate(zip(xs, idx)):
+            with torch.cuda.stream(streams[j % 2]):
+                got.append((j, m(x), glu(x, i)))
+    torch.cuda.synchronize()
+    for j, a, b in got:
+        assert torch.equal(a, alone[j][0]) and torch.equal(b, alone[j][1])
 
 
 @pytest.mark.gpu
