@@ -195,9 +195,12 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 __device__ __forceinline__ void cluster_arrive_wait() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
 }
 
@@ -302,7 +305,7 @@ constexpr int kCtlRegs = 56, kEpiRegs = 104;   // setmaxnreg: 128 x 56 + 512 x 1
 constexpr int kGroup = 4, kSlots = 3;          // scale blocks of a staged slot, and the slots
 constexpr int kMaxStages = 8;
 constexpr int kRingBytes = 160 * 1024;
-constexpr int kPartPitch = 257;                // floats of a row of partial sums (kSplit)
+constexpr int kPartPitch = 260;                // floats of a row of partial sums (kSplit)
 constexpr int kPatch = 2048;                   // an epilogue warp's output staging: 32 rows of 64 bytes
 constexpr size_t kSmem = 1024 + kRingBytes + kEpiWarps * kPatch;
 
@@ -694,18 +697,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int n0 = t.nt * kOutCols + part * (kOutCols / 4);   // its first output column
             if (SPLIT) {
-                // the ring is idle: this CTA's sums, [row][column], rows at
-                // a pitch of 257 so that lanes (rows) meet no bank twice and
-                // the others read a row's columns in whole lines
+                // the ring is idle: this CTA's sums, [row][column]. At a pitch
+                // of 65 x 16 bytes neither the lanes' 16-byte pieces of their
+                // rows nor a row's 16-byte pieces meet in a bank.
                 float *sums = reinterpret_cast<float *>(smem_raw + (sbase - smem_u32(smem_raw)));
                 if (row < bm) {
                     float *to = sums + row * kPartPitch;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const int c = (j < 16 ? col0 : col1 - 32) + 2 * j;
-                        to[c] = lo2(acc[j]);
-                        to[c + 1] = hi2(acc[j]);
-                    }
+                    for (int j = 0; j < 32; j += 2)
+                        *reinterpret_cast<ulonglong2 *>(to + (j < 16 ? col0 : col1 - 32) + 2 * j) =
+                            make_ulonglong2(acc[j], acc[j + 1]);
                 }
             } else if (GLU) {
                 // 32 activations of the token's group of 128; the largest of
@@ -770,8 +771,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (SPLIT) {
-            // Each CTA adds up and stores its share of the tile: a warp takes 32
-            // columns of a row, or (gate/up) a row's 128 activations.
+            // Each CTA adds up and stores its share of the tile: a warp takes a
+            // row's 128 activations (gate/up) or 128 columns of a row, a lane
+            // four of them.
             cluster_arrive_wait();
             if (first < tiles) {
                 const Tile t = locate(a, s_g, first, ntiles, tile_rows);
@@ -779,68 +781,75 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t peer[8];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) peer[c] = map_cluster(sbase, min(c, S - 1));
-                // the cluster's sums of N (row, column)s, every load in flight
-                // before the first is used
+                // the cluster's sums from N places, every load in flight before
+                // the first is used
                 auto sums = [&](auto &v, const auto &at) {
-                    constexpr int N = sizeof(v) / sizeof(float);
-                    float x[N][8];
+                    constexpr int N = sizeof(v) / sizeof(float4);
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        if (c < S)
+                    for (int n = 0; n < N; ++n) v[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                            for (int n = 0; n < N; ++n) x[n][c] = ld_cluster(peer[c] + 4 * at(n));
+                    for (int h = 0; h < 2; ++h) {
+                        float4 x[N][4];
 #pragma unroll
-                    for (int n = 0; n < N; ++n) v[n] = 0.0f;
+                        for (int c = 0; c < 4; ++c)
+                            if (4 * h + c < S)
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        if (c < S)
+                                for (int n = 0; n < N; ++n) x[n][c] = ld_cluster4(peer[4 * h + c] + 4 * at(n));
 #pragma unroll
-                            for (int n = 0; n < N; ++n) v[n] += x[n][c];
+                        for (int c = 0; c < 4; ++c)
+                            if (4 * h + c < S)
+#pragma unroll
+                                for (int n = 0; n < N; ++n) {
+                                    v[n].x += x[n][c].x;
+                                    v[n].y += x[n][c].y;
+                                    v[n].z += x[n][c].z;
+                                    v[n].w += x[n][c].w;
+                                }
+                    }
                 };
                 if (GLU) {
+                    const int c = 4 * lane, n = t.nt * 128 + c;
                     for (int u = (warp - 4) * S + rank; u < np; u += kEpiWarps * S) {
-                        float g[8], v[4];            // gate and up of this lane's four columns
-                        uint32_t m = 0;
-                        sums(g, [&](int n) {
-                            const int c = lane + 32 * (n & 3);
-                            return u * kPartPitch + (c >> 6) * 128 + (c & 63) + 64 * (n >> 2);
-                        });
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t y = glu_pair(g[i], 0.0f, g[4 + i], 0.0f, a.act);
-                            v[i] = bf_lo(y);
-                            if (t.nt * 128 + lane + 32 * i < a.N) m = max(m, y & 0x7FFFu);
-                        }
-                        const QScale qs = qscale(__reduce_max_sync(0xffffffffu, m));
+                        float4 g[2];             // gate and up of this lane's four columns
+                        sums(g, [&](int i) { return u * kPartPitch + (c >> 6) * 128 + (c & 63) + 64 * i; });
+                        const uint32_t y0 = glu_pair(g[0].x, g[0].y, g[1].x, g[1].y, a.act);
+                        const uint32_t y1 = glu_pair(g[0].z, g[0].w, g[1].z, g[1].w, a.act);
+                        uint32_t m = n < a.N ? __vmaxu2(y0 & 0x7FFF7FFFu, y1 & 0x7FFF7FFFu) : 0u;
+                        m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+                        const QScale qs = qscale(m);
                         const size_t r = (size_t)(t.row0 + u);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int n = t.nt * 128 + lane + 32 * i;
-                            if (n < a.N) a.q_out[r * a.N + n] = (uint8_t)cvt_e4m3x2(quotient(v[i], qs), 0.0f);
-                        }
+                        if (n < a.N)
+                            *reinterpret_cast<uint32_t *>(a.q_out + r * a.N + n) =
+                                cvt_e4m3x2(quotient(bf_lo(y0), qs), quotient(bf_hi(y0), qs)) |
+                                (cvt_e4m3x2(quotient(bf_lo(y1), qs), quotient(bf_hi(y1), qs)) << 16);
                         if (lane == 0) a.s_out[(size_t)t.nt * a.P + r] = qs.s;
                     }
                 } else {
-                    // 32 columns of a row a warp and step, four steps at a time
-                    constexpr int kSteps = 4;
-                    const int stride = kEpiWarps * S, total = 8 * np;
+                    // two steps at a time
+                    constexpr int kSteps = 2;
+                    const int stride = kEpiWarps * S, total = 2 * np;
                     for (int u0 = (warp - 4) * S + rank; u0 < total; u0 += kSteps * stride) {
-                        float v[kSteps];
-                        sums(v, [&](int n) {
-                            const int u = min(u0 + n * stride, total - 1);
-                            return (u >> 3) * kPartPitch + (u & 7) * 32 + lane;
+                        float4 v[kSteps];
+                        sums(v, [&](int i) {
+                            const int u = min(u0 + i * stride, total - 1);
+                            return (u >> 1) * kPartPitch + (u & 1) * 128 + 4 * lane;
                         });
 #pragma unroll
                         for (int k = 0; k < kSteps; ++k) {
-                            const int u = u0 + k * stride, n = t.nt * 256 + (u & 7) * 32 + lane;
+                            const int u = u0 + k * stride, n = t.nt * 256 + (u & 1) * 128 + 4 * lane;
                             if (u >= total || n >= a.N) continue;
-                            const int r = t.row0 + (u >> 3), o = a.map ? a.map[r] : r;
+                            const int r = t.row0 + (u >> 1), o = a.map ? a.map[r] : r;
                             if (a.out_f32) {
-                                static_cast<float *>(a.out)[o * a.out_stride + n] = v[k];
+                                *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + o * a.out_stride + n) = v[k];
                             } else {
-                                float y = bf16r(v[k]);
-                                if (a.row_scale) y = bf16r(y * a.row_scale[o]);
-                                static_cast<uint16_t *>(a.out)[o * a.out_stride + n] = f32_to_bf16(y);
+                                uint32_t y0 = cvt_bf16x2(v[k].x, v[k].y), y1 = cvt_bf16x2(v[k].z, v[k].w);
+                                if (a.row_scale) {
+                                    const float rs = a.row_scale[o];
+                                    y0 = cvt_bf16x2(bf_lo(y0) * rs, bf_hi(y0) * rs);
+                                    y1 = cvt_bf16x2(bf_lo(y1) * rs, bf_hi(y1) * rs);
+                                }
+                                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + o * a.out_stride + n) =
+                                    make_uint2(y0, y1);
                             }
                         }
                     }
@@ -1272,7 +1281,7 @@ vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const voi
                 const int slots = max_clusters(kernel_of<kSplit>(glu, fp8), s);
                 if (tiles_of(bm) <= slots)
                     consider(kSplit, bm, s, bm == 32 ? 0.45 : bm == 64 ? 0.5 : 0.55,
-                             3.5 + 0.01 * bm + 0.1 * bm / s, slots);
+                             3.5 + 0.01 * bm + 0.006 * bm * s, slots);
             }
     const int stage = p.bm * 128 + (mode == kPair ? 128 : 256) * 128;
     p.stages = std::min(kMaxStages, kRingBytes / stage);
