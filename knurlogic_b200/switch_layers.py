@@ -426,8 +426,9 @@ class Fp8SwitchLinear(Fp8Buffers, _SwitchBase):
         return self.weight.shape[2]
 
     def descriptor(self) -> _lib.Linear:
-        require_cuda(self.weight, self.weight_scale_inv)
-        return _lib.Linear.from_buffer_copy(fp8_descriptor(self, self.weight.shape[0]))
+        w = self._buffers["weight"]
+        require_cuda(w, self._buffers["weight_scale_inv"])
+        return fp8_descriptor(self, w.shape[0])
 
 
 class SwiGLU(nn.Module):
@@ -462,24 +463,27 @@ class SwitchGLU(nn.Module):
     def gate_descriptor(self) -> _lib.Linear:
         """The gate linear's descriptor, naming the activation."""
         g = self.gate_proj.descriptor()
-        g.activation = self.activation.code
+        code = self.activation.code
+        if g.activation != code:
+            g = _lib.Linear.from_buffer_copy(g)     # a module may keep the one it gives
+            g.activation = code
         return g
 
     def forward(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
         require_cuda(x, indices)
         if x.dtype != torch.bfloat16:
             raise TypeError(f"x must be bfloat16, got {x.dtype}")
-        H = self.gate_proj.input_dims
+        m = self._modules
+        g, u, d = self.gate_descriptor(), m["up_proj"].descriptor(), m["down_proj"].descriptor()
+        H = g.in_features
         k = indices.shape[-1]
         lead = indices.shape[:-1]
         xi = _contig(x.reshape(-1, H))
         T = xi.shape[0]
         ii = _contig(indices.reshape(T, k).to(torch.int32))
-        y = torch.empty((T, k, self.down_proj.output_dims), dtype=torch.bfloat16,
-                        device=x.device)
-        g, u, d = self.gate_descriptor(), self.up_proj.descriptor(), self.down_proj.descriptor()
+        y = x.new_empty((T, k, d.out_features))
         ws_bytes = _lib.lib().vqmoe_switch_glu_workspace_size(ctypes_ref(g), ctypes_ref(d), T, k)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
         _lib.call("vqmoe_switch_glu", ctypes_ref(g), ctypes_ref(u), ctypes_ref(d),
                   xi.data_ptr(), ii.data_ptr(), T, k, y.data_ptr(), ws.data_ptr(),
                   ws_bytes, _stream(x))
