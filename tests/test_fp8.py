@@ -17,8 +17,8 @@ import numpy as np
 import pytest
 import torch
 
-from knurlogic_b200 import (Fp8Linear, Fp8SwitchLinear, SparseMoeBlock, SwitchGLU, _lib, fp8, grouped_linear,
-                            quantize_fp8, synth, tensor_split)
+from knurlogic_b200 import (Fp8Linear, Fp8SwitchLinear, SparseMoeBlock, SwitchGLU, _lib, fp8, gemma4,
+                            grouped_linear, quantize_fp8, synth, tensor_split)
 from knurlogic_b200.switch_layers import GeGLU
 from oracle import moe_ref as R
 from tests.conftest import assert_bf16_close, to_np
@@ -227,7 +227,7 @@ def linear_64(x, w, s):
 
 LINEAR = [(1, 16, 16), (1, 4096, 2048), (2, 128, 128), (3, 144, 272), (16, 256, 4096), (17, 272, 1360), (33, 528, 512),
           (64, 1024, 2048), (65, 400, 144), (100, 2048, 640), (128, 256, 2000), (129, 272, 2000), (300, 528, 384),
-          (257, 16, 128), (640, 768, 1040)]
+          (257, 16, 128), (640, 768, 1040), (2600, 2064, 528)]
 
 
 @pytest.mark.gpu
@@ -360,7 +360,9 @@ GROUPED = [("uniform", 4, 1, 16, 16), ("uniform", 8, 40, 144, 272), ("skew", 16,
            ("uniform", 1, 129, 256, 144), ("uniform", 1024, 700, 16, 64), ("none", 6, 12, 32, 32),
            ("one", 200, 17, 720, 1360), ("skew", 3, 1500, 400, 1040),
            # several tiles a CTA, more scale blocks than accumulators
-           ("uniform", 128, 600, 768, 1168), ("skew", 100, 2000, 640, 2064)]
+           ("uniform", 128, 600, 768, 1168), ("skew", 100, 2000, 640, 2064),
+           # many rows a group: CTA pairs, the last pair half empty
+           ("skew", 2, 1500, 400, 1040), ("uniform", 2, 1410, 1296, 272)]
 
 
 @pytest.mark.gpu
@@ -464,7 +466,9 @@ def experts_64(x, idx, gate, up, down, kind="swiglu"):
 
 EXPERTS = [(1, 8, 2, 256, 128), (1, 64, 8, 2048, 768), (3, 16, 4, 272, 144), (24, 16, 4, 512, 256),
            (64, 64, 8, 640, 384), (300, 8, 2, 400, 272), (700, 4, 3, 256, 144), (2100, 8, 2, 128, 128),
-           (40, 200, 1, 144, 400), (60, 128, 8, 1168, 384)]
+           (40, 200, 1, 144, 400), (60, 128, 8, 1168, 384),
+           # the smallest widths, more experts a token than eight, CTA pairs
+           (2, 8, 2, 16, 16), (5, 16, 9, 64, 16), (40, 40, 32, 128, 32), (900, 2, 2, 272, 144)]
 
 
 @pytest.mark.gpu
@@ -482,6 +486,23 @@ def test_switch_glu_matches_64_bits(T, E, k, H, I):
     assert y.shape == (T, k, H)
     ref = experts_64(f64(x), idx, gate, up, down, kind)
     assert_bf16_close(to_np(y), ref, f"fp8 glu T{T} E{E} k{k} H{H} I{I}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 8, 4, 256, 128), (50, 8, 2, 400, 144), (700, 4, 2, 272, 256),
+                                       (1500, 4, 2, 272, 256)])
+def test_weighted_experts_match_64_bits(T, E, k, H, I):
+    """Gemma-4's `Experts` in the format: bf16(y * w) a pair, summed over the
+    slots in float32 and rounded once."""
+    gate, up, down = make_weight((E, I, H), 4, DEV), make_weight((E, I, H), 5, DEV), make_weight((E, H, I), 6, DEV)
+    m = gemma4.Experts(SwitchGLU(*(Fp8SwitchLinear(*w) for w in (gate, up, down)), activation=GeGLU()))
+    x = make_x(T, H, T, DEV)
+    rng = np.random.default_rng(T)
+    idx = np.stack([rng.choice(E, k, replace=False) for _ in range(T)]).astype(np.int32)
+    w = bf(rng.random((T, k)) + 0.1)
+    out = m(x, torch.from_numpy(idx).to(DEV), torch.from_numpy(w).to(torch.bfloat16).to(DEV))
+    ref = R.combine(experts_64(f64(x), idx, gate, up, down, "geglu"), w)
+    assert_bf16_close(to_np(out), ref, f"fp8 weighted experts T{T}")
 
 
 @pytest.mark.gpu
