@@ -131,6 +131,8 @@ class Fp8Linear(Fp8Buffers, nn.Module):
     scales applied to each block's sum, and rounded once to bf16 (or kept as
     float32, for logits)."""
 
+    weight_dims = 2
+
     def __init__(self, weight: torch.Tensor, weight_scale_inv: torch.Tensor):
         super().__init__()
         check_fp8_weight(weight, weight_scale_inv, 2)
@@ -148,7 +150,7 @@ class Fp8Linear(Fp8Buffers, nn.Module):
     def descriptor(self) -> _lib.Linear:
         w = self.weight
         require_cuda(w, self.weight_scale_inv)
-        return fp8_descriptor(self, 1)
+        return fp8_descriptor(self)
 
     def forward(self, x: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         if out_dtype not in (torch.bfloat16, torch.float32):
@@ -159,7 +161,7 @@ class Fp8Linear(Fp8Buffers, nn.Module):
         if w.device != x.device:
             _same_device(x, weight=w)
         out = x.new_empty((*x.shape[:-1], N), dtype=out_dtype)
-        return _run(fp8_descriptor(self, 1), xr, None, out)
+        return _run(fp8_descriptor(self), xr, None, out)
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,

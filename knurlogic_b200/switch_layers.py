@@ -373,27 +373,49 @@ def check_fp8_weight(weight: torch.Tensor, scales: torch.Tensor, dims: int) -> N
                          f"{tuple(weight.shape)} is {shape}")
 
 
-def fp8_descriptor(module: nn.Module, experts: int) -> _lib.Linear:
-    """The descriptor of a module's `weight` and `weight_scale_inv`, built
-    again when either lies elsewhere (the caller changes nothing in it)."""
+def fp8_descriptor(module: Fp8Buffers) -> _lib.Linear:
+    """The descriptor of a module's `weight` and `weight_scale_inv`, which
+    are checked and described again whenever either differs in anything the
+    kernels go by: a buffer can be replaced by a view of its own beginning,
+    or by one of another shape where the last one lay (the caller changes
+    nothing in the descriptor)."""
     w, s = module._buffers["weight"], module._buffers["weight_scale_inv"]
-    wp, sp = w.data_ptr(), s.data_ptr()
-    d = module.__dict__.get("_descriptor")
-    if d is None or d.weight != wp or d.scales != sp:
-        d = _lib.Linear(format=_lib.FMT_FP8_BLOCK, num_experts=experts, out_features=w.shape[-2],
-                        in_features=w.shape[-1], weight=wp, scales=sp, group_size=128)
-        module.__dict__["_descriptor"] = d
-    return d
+    key = (w.data_ptr(), s.data_ptr(), w.shape, s.shape, w.dtype, s.dtype, w.device, s.device, w.is_contiguous(),
+           s.is_contiguous())
+    held = module.__dict__.get("_descriptor")
+    if held is None or held[0] != key:
+        check_fp8_weight(w, s, module.weight_dims)
+        if s.dtype != torch.float32:
+            raise ValueError(f"weight_scale_inv must be float32, got {s.dtype}")
+        if s.device != w.device:
+            raise ValueError(f"weight_scale_inv is on {s.device}, weight on {w.device}")
+        if not (w.is_contiguous() and s.is_contiguous()):
+            raise ValueError("weight and weight_scale_inv must be contiguous")
+        held = key, _lib.Linear(format=_lib.FMT_FP8_BLOCK, num_experts=w.shape[0] if w.dim() == 3 else 1,
+                                out_features=w.shape[-2], in_features=w.shape[-1], weight=key[0], scales=key[1],
+                                group_size=128)
+        module.__dict__["_descriptor"] = held
+    return held[1]
 
 
 class Fp8Buffers:
     """Modules with an `fp8_descriptor`: it holds addresses, so copies and
-    pickles leave it out."""
+    pickles leave it out; and a cast of the model (`.to(dtype)`, `.half()`)
+    moves the e4m3 weights and their float32 scales but converts neither --
+    torch counts both among a module's floating-point buffers."""
+
+    weight_dims: int                      # of `weight`: 3 with the experts', else 2
 
     def __getstate__(self):
         d = self.__dict__.copy()
         d.pop("_descriptor", None)
         return d
+
+    def _apply(self, fn, *args, **kwargs):
+        def place(t):
+            r = fn(t)
+            return r if r.dtype == t.dtype else t.to(r.device)
+        return super()._apply(place, *args, **kwargs)
 
 
 class Fp8SwitchLinear(Fp8Buffers, _SwitchBase):
@@ -406,6 +428,8 @@ class Fp8SwitchLinear(Fp8Buffers, _SwitchBase):
     float32 scale for each row and 128 inputs), the products are summed in
     float32 and the output rounded once to bf16. In a `SwitchGLU` the
     activations between gate/up and down are quantized the same way."""
+
+    weight_dims = 3
 
     def __init__(self, weight: torch.Tensor, weight_scale_inv: torch.Tensor):
         super().__init__()
@@ -428,7 +452,7 @@ class Fp8SwitchLinear(Fp8Buffers, _SwitchBase):
     def descriptor(self) -> _lib.Linear:
         w = self._buffers["weight"]
         require_cuda(w, self._buffers["weight_scale_inv"])
-        return fp8_descriptor(self, w.shape[0])
+        return fp8_descriptor(self)
 
 
 class SwiGLU(nn.Module):
