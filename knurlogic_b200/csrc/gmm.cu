@@ -402,6 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
+    // warp 0 uses `full` before the CTA's barrier (the early weights below), by
+    // an elected lane that need not be the one that initialised it
+    __syncwarp();
     if (warp == 1) {
         if (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)),
