@@ -469,7 +469,8 @@ VQMOE_API vqmoe_status vqmoe_quantize_fp8(const void *x, int64_t rows, int32_t c
 
 /* Rows in group order times their group's weights: out[r] = x[r] @ W[e]^T for
  * offsets[e] <= r < offsets[e+1] (device int32 [E+1], ascending; values
- * outside [0, rows] are clamped). w: DENSE_BF16 or FP8_BLOCK, E <= 1024; with
+ * outside [0, rows] are clamped, and one below an earlier offset counts as
+ * the largest before it). w: DENSE_BF16 or FP8_BLOCK, E <= 1024; with
  * FP8_BLOCK the rows are quantized as vqmoe_quantize_fp8 does, into the
  * workspace. offsets null: one group of all rows (E == 1), a dense linear.
  * Rows of out that lie in no group are left as they were. x bf16, rows at a

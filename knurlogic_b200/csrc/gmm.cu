@@ -215,17 +215,33 @@ struct Groups {
     int beg[kMaxGroups], end[kMaxGroups];
 };
 
-// Warp 0 fills the groups' rows, clamped to [0, P] and to ascending order
-// whatever the offsets hold, and the running count of their token tiles.
+// Warp 0 fills the groups' rows and the running count of their token tiles.
+// Whatever the offsets hold, group e has the rows between the largest of the
+// first e + 1 offsets and of the first e + 2, all clamped to [0, P]: groups
+// never share a row (two tiles would write it, in no order), and their tiles
+// are at most the launcher's bound (a cluster of kSplit takes one tile).
 __device__ __forceinline__ void build_groups(const GmmArgs &a, Groups &g, int rows_per_tile) {
     const int lane = threadIdx.x & 31;
-    const int per = (a.E + 31) / 32, e0 = lane * per;
+    const int per = (a.E + 31) / 32, e0 = lane * per, e1 = min(e0 + per, a.E);
+    auto tiles = [&](int e) { return (g.end[e] - g.beg[e] + rows_per_tile - 1) / rows_per_tile; };
     int sum = 0;
-    for (int e = e0; e < min(e0 + per, a.E); ++e) {
-        const int b = min(max(__ldg(a.off + e), 0), a.P), n = min(max(__ldg(a.off + e + 1), b), a.P);
+    bool falls = false;
+    for (int e = e0; e < e1; ++e) {
+        const int b = min(max(__ldg(a.off + e), 0), a.P), n = min(max(__ldg(a.off + e + 1), 0), a.P);
+        falls |= n < b;
         g.beg[e] = b;
         g.end[e] = n;
         sum += (n - b + rows_per_tile - 1) / rows_per_tile;
+    }
+    if (__any_sync(0xffffffffu, falls)) {          // not as documented: the running maximum, by one lane
+        if (lane == 0)
+            for (int e = 0, most = g.beg[0]; e < a.E; ++e) {
+                g.beg[e] = most;
+                g.end[e] = most = max(most, g.end[e]);
+            }
+        __syncwarp();
+        sum = 0;
+        for (int e = e0; e < e1; ++e) sum += tiles(e);
     }
     int inc = sum;
 #pragma unroll
@@ -234,9 +250,9 @@ __device__ __forceinline__ void build_groups(const GmmArgs &a, Groups &g, int ro
         if (lane >= o) inc += v;
     }
     int at = inc - sum;
-    for (int e = e0; e < min(e0 + per, a.E); ++e) {
+    for (int e = e0; e < e1; ++e) {
         g.pre[e] = at;
-        at += (g.end[e] - g.beg[e] + rows_per_tile - 1) / rows_per_tile;
+        at += tiles(e);
     }
     if (lane == 31) g.pre[a.E] = inc;
 }

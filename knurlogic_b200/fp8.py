@@ -173,8 +173,10 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     x [P, IN] bf16 (rows may lie at a pitch); weight [E, OUT, IN] bf16, or
     float8_e4m3fn with `weight_scale_inv [E, ceil(OUT/128), ceil(IN/128)]`
     float32 (x is then quantized as by `quantize_fp8`); offsets [E + 1] int32
-    on the device, ascending; E <= 1024, OUT and IN multiples of 16. Sums are
-    float32, rounded once to `out_dtype` (bf16 or float32). Rows that lie in no
+    on the device, ascending (not read on the host: values outside [0, P] are
+    clamped, one below an earlier offset counts as the largest before it);
+    E <= 1024, OUT and IN multiples of 16. Sums are float32, rounded once to
+    `out_dtype` (bf16 or float32). Rows that lie in no
     group -- before the first offset or behind the last -- are left as they
     were in `out` (contiguous [P, OUT]); without `out` they are unset."""
     require_cuda(x, weight, offsets, weight_scale_inv, out)
