@@ -150,13 +150,16 @@ def _sigmoid_bf16(x: torch.Tensor) -> torch.Tensor:
     return torch.sigmoid(x.float()).to(torch.bfloat16)
 
 
-def _linear(w: dict, name: str):
-    """The projection `{name}.weight` of a state dict as a function of x:
-    block-scaled e4m3 (`{name}.weight_scale_inv` beside it) or bf16."""
+def _projection(w: dict, name: str):
+    """The projection `{name}.weight` of a state dict: an `Fp8Linear` where
+    it is block-scaled e4m3 (`{name}.weight_scale_inv` beside it), else the
+    bf16 weight itself."""
     wt, sc = w[name + ".weight"], w.get(name + ".weight_scale_inv")
-    if sc is not None:
-        return Fp8Linear(wt, sc)
-    return lambda x: F.linear(x, wt)
+    return wt if sc is None else Fp8Linear(wt, sc)
+
+
+def _project(x: torch.Tensor, p) -> torch.Tensor:
+    return F.linear(x, p) if torch.is_tensor(p) else p(x)
 
 
 # --------------------------------------------------------------- attention
@@ -206,7 +209,7 @@ class Attention:
 
     def __init__(self, w: dict, p: str, cfg: DecoderConfig):
         self.cfg = cfg
-        self.wq, self.wk, self.wv, self.wo = (_linear(w, p + n) for n in ("q_proj", "k_proj", "v_proj", "o_proj"))
+        self.wq, self.wk, self.wv, self.wo = (_projection(w, p + n) for n in ("q_proj", "k_proj", "v_proj", "o_proj"))
         self.q_norm = _gain(w[p + "q_norm.weight"])
         self.k_norm = _gain(w[p + "k_norm.weight"])
 
@@ -217,11 +220,11 @@ class Attention:
         c = self.cfg
         B, L, _ = x.shape
         nh, kv, d = c.heads, c.kv_heads, c.head_dim
-        q = self.wq(x).view(B, L, nh, 2 * d)
+        q = _project(x, self.wq).view(B, L, nh, 2 * d)
         queries = add_rms_norm(q[..., :d].contiguous(), None, self.q_norm, c.eps)
         gate = q[..., d:].reshape(B, L, nh * d)
-        keys = add_rms_norm(self.wk(x).view(B, L, kv, d), None, self.k_norm, c.eps)
-        values = self.wv(x).view(B, L, kv, d)
+        keys = add_rms_norm(_project(x, self.wk).view(B, L, kv, d), None, self.k_norm, c.eps)
+        values = _project(x, self.wv).view(B, L, kv, d)
         queries = rope(queries, pos0, c.rotary_dims, c.rope_theta)
         keys = rope(keys, pos0, c.rotary_dims, c.rope_theta)
         rep = nh // kv
@@ -234,7 +237,7 @@ class Attention:
             o = F.scaled_dot_product_attention(Q, cache.k.transpose(1, 2), cache.v.transpose(1, 2), attn_mask=mask,
                                                scale=d ** -0.5)
             o = o.view(B, kv, rep, L, d).permute(0, 3, 1, 2, 4).reshape(B, L, nh * d)
-            return self.wo(o * _sigmoid_bf16(gate))
+            return _project(o * _sigmoid_bf16(gate), self.wo)
         if pos0 + L > cache.max_len:
             raise ValueError(f"KV cache of {cache.max_len} positions: writing {pos0}..{pos0 + L}")
         cache.k[:, pos0:pos0 + L] = keys
@@ -258,7 +261,7 @@ class Attention:
                 o = F.scaled_dot_product_attention(Q, K, V, attn_mask=mask, scale=d ** -0.5)
             o = o.view(B, kv, rep, L, d).permute(0, 3, 1, 2, 4)
         o = o.reshape(B, L, nh * d)
-        return self.wo(o * _sigmoid_bf16(gate))
+        return _project(o * _sigmoid_bf16(gate), self.wo)
 
 
 class DecoderLayer:
