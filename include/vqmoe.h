@@ -180,7 +180,9 @@ typedef struct {
     int32_t router_mode;         /* VQMOE_ROUTER_* (0: Qwen3.5) */
     int32_t wait_polls;          /* polls before a phase 2 tile gives up waiting
                                     for its expert's phase 1 tiles; 0: the
-                                    default (about four seconds) */
+                                    default (about four seconds). VQ_REF, AFFINE
+                                    and FP8_BLOCK experts have no such wait:
+                                    their phases are separate launches */
 } vqmoe_block;
 
 /* Output dtype of vqmoe_sparse_moe_block. F32 holds the bf16 block output

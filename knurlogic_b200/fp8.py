@@ -27,10 +27,14 @@ _status: dict = {}
 
 def _status_word(device: torch.device) -> torch.Tensor | None:
     """The device's word that a bounded wait raises when it runs out. None
-    inside a stream capture that comes before any other call."""
+    inside a stream capture that no call and no module on the device came
+    before (a word made there would be the graph's own)."""
     w = _status.get(device.index)
     if w is None and not torch.cuda.is_current_stream_capturing():
-        w = _status[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):                    # cleared in any mode later
+            w = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()      # zero before another stream's kernels see it
+        w = _status.setdefault(device.index, w)
     return w
 
 
@@ -138,6 +142,18 @@ class Fp8Linear(Fp8Buffers, nn.Module):
         check_fp8_weight(weight, weight_scale_inv, 2)
         self.register_buffer("weight", weight.contiguous())
         self.register_buffer("weight_scale_inv", weight_scale_inv.to(torch.float32).contiguous())
+        self._report()
+
+    def _report(self) -> None:
+        """The device has its status word before the module's first call,
+        which may be captured."""
+        if self.weight.is_cuda:
+            _status_word(self.weight.device)
+
+    def _apply(self, *args, **kwargs):
+        r = super()._apply(*args, **kwargs)
+        self._report()
+        return r
 
     @property
     def out_features(self):

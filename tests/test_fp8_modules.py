@@ -4,9 +4,11 @@ import pytest
 import torch
 from torch import nn
 
-from knurlogic_b200 import Fp8Linear, Fp8SwitchLinear
+from knurlogic_b200 import Fp8Linear, Fp8SwitchLinear, fp8, grouped_linear
 from knurlogic_b200.switch_layers import fp8_descriptor
-from tests.test_fp8 import make_weight
+from tests.test_fp8 import make_weight, make_x
+
+DEV = "cuda:0"
 
 MODULES = [(Fp8Linear, (256, 384)), (Fp8SwitchLinear, (2, 256, 384))]
 
@@ -83,3 +85,81 @@ def test_a_state_dict_assigned_in_another_type_is_refused():
     m.load_state_dict({k: v.to(torch.bfloat16) for k, v in o.state_dict().items()}, assign=True)
     with pytest.raises(ValueError, match="float8_e4m3fn"):
         fp8_descriptor(m)
+
+
+# ------------------------------------------------------------------ GPU
+# The kernels' own waits cannot be made to run out without a fault, so the
+# tests raise the device's word themselves, by an ordinary copy.
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_a_wait_that_ran_out_is_reported_once(monkeypatch, mode):
+    monkeypatch.setattr(fp8, "_status", {})
+    with mode():
+        m = Fp8Linear(*make_weight((144, 272), 1, DEV))
+        x = make_x(3, 272, 1, DEV)
+        y = m(x)
+        fp8.check_status(DEV)
+        fp8._status[0].fill_(1)
+        m(x)                                            # a later call does not clear it
+    with pytest.raises(TimeoutError, match="ran out"):
+        fp8.check_status()
+    fp8.check_status(DEV)
+    assert torch.equal(m(x), y)
+    fp8.check_status(torch.device(DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("place", [lambda: Fp8Linear(*make_weight((144, 272), 1, DEV)),
+                                   lambda: Fp8Linear(*make_weight((144, 272), 1)).to(DEV)], ids=["made", "moved"])
+def test_a_captured_first_call_has_a_status_word(monkeypatch, place):
+    """A module's device has its word before the first call on it, which may
+    be a captured one: the graph's kernels are given it."""
+    monkeypatch.setattr(fp8, "_status", {})
+    m, x = place(), make_x(3, 272, 1, DEV)
+    assert list(fp8._status) == [0]
+    given = []
+    call = fp8._call_on
+    monkeypatch.setattr(fp8, "_call_on", lambda dev, name, *a: (given.append(a[-1]), call(dev, name, *a)))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = m(x)
+    g.replay()
+    assert given == [fp8._status[0].data_ptr()]
+    assert torch.equal(y, m(x))
+
+
+@pytest.mark.gpu
+def test_a_captured_first_grouped_call_runs_without_one(monkeypatch):
+    """No module came before it: the call is captured all the same, with no
+    word to raise, and leaves none of the graph's memory behind as one."""
+    w = torch.randn(3, 32, 64, device=DEV).to(torch.bfloat16)
+    x, off = make_x(50, 64, 1, DEV), torch.tensor([0, 10, 10, 50], dtype=torch.int32, device=DEV)
+    ref = grouped_linear(x, w, off)
+    monkeypatch.setattr(fp8, "_status", {})
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = grouped_linear(x, w, off)
+    g.replay()
+    assert torch.equal(y, ref) and not fp8._status
+    fp8.check_status(DEV)
+
+
+@pytest.mark.gpu
+def test_a_cast_model_gives_the_same_product():
+    m, x = Fp8Linear(*make_weight((144, 272), 1, DEV)), make_x(5, 272, 2, DEV)
+    y = m(x)
+    assert torch.equal(m.to(torch.bfloat16)(x), y) and torch.equal(m.cpu().half().to(DEV)(x), y)
+
+
+@pytest.mark.gpu
+def test_a_product_follows_replaced_buffers():
+    """The first 128 outputs, from a view of the weights' beginning, and
+    nothing written behind them."""
+    m, x = Fp8Linear(*make_weight((400, 272), 1, DEV)), make_x(5, 272, 2, DEV)
+    y = m(x)
+    m.weight, m.weight_scale_inv = m.weight[:128], m.weight_scale_inv[:1]
+    assert torch.equal(m(x), y[:, :128])
+    m.weight = m.weight.to(torch.bfloat16)
+    with pytest.raises(ValueError, match="float8_e4m3fn"):
+        m(x)
