@@ -516,7 +516,10 @@ def generate_mtp(model: TextModel, prompts: torch.Tensor, steps: int, k: int = 3
     graphs: the verify, the head's catch-up and its one-row draft each
     replay as one CUDA graph; one host read per step (m).
     Returns (tokens [B, steps], {"steps", "drafted", "accepted",
-    "prefill_ms", "decode_ms"}); the tokens are plain greedy decoding's."""
+    "prefill_ms", "decode_ms"}); the tokens are plain greedy decoding's, but
+    for near-ties: a (k+1)-wide forward may add a projection's float32 sum in
+    another order than a 1-wide one (cuBLAS's choice of kernel, or
+    `Fp8Linear`'s), and two logits within that rounding then change places."""
     if model.mtp is None:
         raise ValueError("the model has no MTP head")
     B, P = prompts.shape

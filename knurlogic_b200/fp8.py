@@ -133,7 +133,8 @@ class Fp8Linear(Fp8Buffers, nn.Module):
     `forward(x [..., IN] bf16, out_dtype=torch.bfloat16)`: the rows are
     quantized (`quantize_fp8`), the products summed in float32 with both
     scales applied to each block's sum, and rounded once to bf16 (or kept as
-    float32, for logits)."""
+    float32, for logits). The order of a row's float32 additions goes by the
+    number of rows in the call, never by their values."""
 
     weight_dims = 2
 
