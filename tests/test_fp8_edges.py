@@ -4,8 +4,10 @@ import numpy as np
 import pytest
 import torch
 
-from knurlogic_b200 import Fp8Linear, fp8, grouped_linear
-from tests.test_fp8 import (check, f64, grouped_64, linear_64, make_weight, make_x, quantize_64, spread, weight_64)
+from knurlogic_b200 import Fp8Linear, Fp8SwitchLinear, SwitchGLU, fp8, grouped_linear, quantize_fp8
+from tests.conftest import assert_bf16_close, to_np
+from tests.test_fp8 import (check, experts_64, f64, grouped_64, linear_64, make_weight, make_x, quantize_64, spread,
+                            weight_64)
 
 DEV = "cuda:0"
 
@@ -58,4 +60,67 @@ def test_offsets_that_fall_back_name_no_row_twice(kind, P, quant):
     assert (out[:a] == 7).all() and (out[b:] == 7).all()
     if a < b:
         check(out[a:b], ref[a:b], mag[a:b], K)
+    fp8.check_status(DEV)
+
+
+def _glu(E, H, I):
+    w = make_weight((E, I, H), 1, DEV), make_weight((E, I, H), 2, DEV), make_weight((E, H, I), 3, DEV)
+    return SwitchGLU(*(Fp8SwitchLinear(*p) for p in w)), w
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E", [8, 1024])
+def test_pairs_of_no_expert_among_many(E):
+    """From 4096 pairs the sort is spread over CTAs: ids outside the experts
+    take no place there either, and an expert named twice by a token has both
+    its pairs."""
+    T, k, H, I = 2100, 3, 64, 32
+    glu, w = _glu(E, H, I)
+    x = make_x(T, H, 1, DEV)
+    idx = np.random.default_rng(E).integers(0, E, (T, k)).astype(np.int32)
+    idx[7] = idx[7, 0]
+    idx[5, 1], idx[6], idx[T - 1, 2] = -1, (E, 1 << 30, -(1 << 31)), E
+    ok = (idx >= 0) & (idx < E)
+    y = to_np(glu(x, torch.from_numpy(idx).to(DEV)))
+    assert np.array_equal(y[7, 0], y[7, 1]) and np.array_equal(y[7, 0], y[7, 2])
+    ref = experts_64(f64(x), idx, *w)
+    assert_bf16_close(y[ok], ref[ok], f"pairs of no expert, {E} experts")
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_a_launch_takes():
+    """8192 tokens a launch: the rest is a launch of its own."""
+    E, k, H, I = 8, 2, 64, 32
+    glu, w = _glu(E, H, I)
+    x = make_x(8200, H, 1, DEV)
+    idx = np.random.default_rng(1).integers(0, E, (8200, k)).astype(np.int32)
+    y = glu(x, torch.from_numpy(idx).to(DEV))
+    assert_bf16_close(to_np(y), experts_64(f64(x), idx, *w), "8200 tokens")
+    rows = glu.down_proj(make_x(8200, I, 2, DEV).view(8200, 1, I), torch.from_numpy(idx[:, 0]).to(DEV)).view(8200, H)
+    q, xs = quantize_64(f64(make_x(8200, I, 2)))
+    xv, wv = q * spread(xs, I), weight_64(f64(w[2][0]), f64(w[2][1]))
+    at = idx[:, 0]
+    check(rows, np.einsum("rk,rnk->rn", xv, wv[at]), np.einsum("rk,rnk->rn", np.abs(xv), np.abs(wv[at])), I)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """More than 2^31 values quantized, and more than 2^31 outputs."""
+    K = 4096
+    x = make_x(64, K, 1, DEV).repeat(8300, 1)                  # 2.18e9 values
+    q, s = quantize_fp8(x)
+    rq, rs = quantize_fp8(x[:64])
+    assert torch.equal(q[-64:].view(torch.uint8), rq.view(torch.uint8)) and torch.equal(s[-64:], rs)
+    del q, s
+    m = Fp8Linear(*make_weight((16, K), 2, DEV))
+    check(m(x)[-64:], *linear_64(x[-64:], m.weight, m.weight_scale_inv), K)
+    del x
+    m = Fp8Linear(*make_weight((65536, 128), 3, DEV))
+    x = make_x(64, 128, 4, DEV).repeat(520, 1)                 # 2.18e9 outputs
+    ref = linear_64(x[-64:], m.weight, m.weight_scale_inv)
+    check(m(x)[-64:], *ref, 128)
+    off = torch.tensor([0, 5, x.shape[0]], dtype=torch.int32, device=DEV)
+    w = torch.stack([m.weight[:32768].view(torch.uint8)] * 2).view(torch.float8_e4m3fn)
+    y = grouped_linear(torch.cat([x, x]), w, off * 2, weight_scale_inv=torch.stack([m.weight_scale_inv[:256]] * 2))
+    check(y[-64:], ref[0][:, :32768], ref[1][:, :32768], 128)
     fp8.check_status(DEV)
