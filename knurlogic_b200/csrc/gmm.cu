@@ -31,11 +31,13 @@
 // and kSmall, a kernel of its own with the weights on the lanes, for groups of
 // a few tokens.
 //
-// Measured (us a call, the quantizer included): linear 8192 x 8192 x 4096 e4m3
-// 295 (1.86 PFLOP/s, 1.13 of the measured bf16 rate; 353 when repeated until
-// the power cap holds the clocks down), of 128 tokens 19, of one 13.5 (33.5 MB);
-// bf16 rows grouped by 128 experts of 768 x 2048, 512 rows 69 (398 MB: 0.88 of
-// the measured copy rate), 32768 rows 135 (103 GFLOP).
+// Measured (us of device time a call, replayed from a CUDA graph, the
+// quantizer included; as calls in a loop in brackets, with the host's part or
+// the power cap where either is more): linear 8192 x 8192 x 4096 e4m3 304 (1.81
+// PFLOP/s, 1.10 of the measured bf16 rate) [343 to 352], of 128 tokens 19.1
+// [20.6], of one, 4096 x 4096, 11.3 [19]; rows grouped by 128 experts of 768 x
+// 2048, bf16: 512 rows 67 (398 MB: 0.91 of the measured copy rate) [68 to 70],
+// 32768 rows by Zipf's law 141 (103 GFLOP) [165]; e4m3: 43 [45] and 130 [149].
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -1203,7 +1205,9 @@ static bool byte_map(CUtensorMap *m, const void *base, size_t rows, size_t row_b
 }
 
 // How many clusters of `size` CTAs of the kernel run at a time (each CTA takes
-// an SM, and a cluster stays inside one GPC), looked up once per device.
+// an SM, and a cluster stays inside one GPC), looked up once per device: every
+// kSplit kernel asks for the same threads, registers and dynamic shared memory,
+// one CTA an SM, so the first one's answer is the others' too.
 static int max_clusters(const void *fn, int size) {
     static std::atomic<int> known[64][9];          // the number + 1
     int dev = 0;
@@ -1283,6 +1287,9 @@ vqmoe_status launch_gmm(const void *x, size_t x_pitch, const void *w0, const voi
         // 147, bf16 146 / 126, 149 / 135; mean 512 e4m3 247 / 232, bf16 235 / 192.
         // e4m3 gate/up with down: mean 4 124 / 143 / 148 / 203, mean 32 156 / 156 /
         // 162 (gate/up by kSmall, down by 128 rows: 148), mean 48 188 / 167 / 166.
+        // The points below are those of the even groups at this one shape: other
+        // widths were not measured against each other, and under Zipf the even
+        // groups' choice can be behind (e4m3 mean 16: kSmall 51, 64 rows 46).
         const int mean = (a.P + groups - 1) / groups;
         if (mean <= (glu ? 40 : fp8 ? 20 : 6)) consider(kSmall, kTok, 1, glu ? 0.74 : 0.37, 0.7, sms);
         else if (mean <= 24) consider(kSingle, 64, 1, 0.55, 3.0, sms);

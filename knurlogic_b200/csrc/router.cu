@@ -810,7 +810,7 @@ vqmoe_status launch_route(const int32_t *inds, int P, int E, int32_t *cnt,
 
 // The same sort spread over CTAs, for many pairs (one CTA takes 35 us for
 // 32768 pairs, its shared-memory atomics and its two passes over them; these
-// two launches 9): each CTA counts its pairs per expert in shared memory and
+// two launches 8): each CTA counts its pairs per expert in shared memory and
 // takes a run of places for each expert from the global count; then every CTA
 // scans the counts and places its pairs. cnt[0 .. E) zero on entry.
 constexpr int kRouteWideThreads = 512;

@@ -51,7 +51,7 @@ def tp_reduce(part: torch.Tensor, group) -> torch.Tensor:
 def dense_weight(w: dict, name: str) -> torch.Tensor:
     """`{name}.weight` as a bf16 matmul takes it: a block-scaled e4m3 one
     (`{name}.weight_scale_inv` beside it, a float32 for each 128 x 128 block)
-    restored to bf16, rounded once."""
+    restored to bf16 (the product in float32, then rounded)."""
     wt, sc = w[name + ".weight"], w.get(name + ".weight_scale_inv")
     if sc is None:
         if wt.dtype == torch.float8_e4m3fn:
