@@ -236,6 +236,7 @@ __device__ __forceinline__ void build_groups(const GmmArgs &a, Groups &g, int ro
         sum += (n - b + rows_per_tile - 1) / rows_per_tile;
     }
     if (__any_sync(0xffffffffu, falls)) {          // not as documented: the running maximum, by one lane
+        __syncwarp();                              // (a vote orders no memory)
         if (lane == 0)
             for (int e = 0, most = g.beg[0]; e < a.E; ++e) {
                 g.beg[e] = most;
