@@ -34,7 +34,7 @@ import torch.nn.functional as F
 from . import _lib, synth
 from .fp8 import Fp8Linear
 from .moe import SparseMoeBlock
-from .switch_layers import c_stream, require_cuda
+from .switch_layers import call_on, require_cuda
 
 
 @dataclass(frozen=True)
@@ -135,9 +135,9 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
     H = x.shape[-1]
     rows = x.numel() // H
     out = torch.empty_like(x)
-    _lib.call("vqmoe_add_rms_norm", x.data_ptr(), residual.data_ptr() if residual is not None else None,
-              weight.data_ptr(), rows, H, ctypes.c_float(eps), sum_out.data_ptr() if sum_out is not None else None,
-              out.data_ptr(), c_stream(x.device))
+    call_on(x.device, "vqmoe_add_rms_norm", x.data_ptr(), residual.data_ptr() if residual is not None else None,
+            weight.data_ptr(), rows, H, ctypes.c_float(eps), sum_out.data_ptr() if sum_out is not None else None,
+            out.data_ptr())
     return out
 
 

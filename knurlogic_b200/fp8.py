@@ -19,7 +19,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .switch_layers import Fp8Buffers, _contig, c_stream, check_fp8_weight, fp8_descriptor, require_cuda
+from .switch_layers import Fp8Buffers, _contig, call_on, check_fp8_weight, fp8_descriptor, require_cuda
 
 GROUP = 128
 _status: dict = {}
@@ -72,16 +72,6 @@ def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """An entry point on `device` and its current stream (the last argument)."""
-    i = device.index
-    if i == torch.cuda.current_device():
-        _lib.call(name, *args, c_stream(device))
-    else:
-        with torch.cuda.device(i):
-            _lib.call(name, *args, c_stream(device))
-
-
 def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [..., K] bf16 -> (q [..., K] float8_e4m3fn, scales [..., ceil(K/128)]
     float32), x ~ q * scale. Of a row's group of 128 inputs (the last one
@@ -97,7 +87,7 @@ def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
          else x.new_empty(x.shape, dtype=torch.float8_e4m3fn))
     s = x.new_empty((*x.shape[:-1], -(-K // GROUP)), dtype=torch.float32)
     if xr.shape[0]:
-        _call_on(x.device, "vqmoe_quantize_fp8", xr.data_ptr(), xr.shape[0], K, _pitch(xr), q.data_ptr(), s.data_ptr())
+        call_on(x.device, "vqmoe_quantize_fp8", xr.data_ptr(), xr.shape[0], K, _pitch(xr), q.data_ptr(), s.data_ptr())
     return q, s
 
 
@@ -112,7 +102,7 @@ def _run(d: _lib.Linear, x: torch.Tensor, offsets, out: torch.Tensor) -> torch.T
     st = _status.get(dev.index)
     if st is None:
         st = _status_word(dev)
-    _call_on(dev, "vqmoe_grouped_linear", d, x.data_ptr(), P, _pitch(x),
+    call_on(dev, "vqmoe_grouped_linear", d, x.data_ptr(), P, _pitch(x),
              offsets.data_ptr() if offsets is not None else None, out.data_ptr(),
              _lib.OUT_F32 if out.dtype is torch.float32 else _lib.OUT_BF16,
              ws.data_ptr() if n else None, n, st.data_ptr() if st is not None else None)

@@ -24,7 +24,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .switch_layers import GeGLU, SwitchGLU, _contig, c_stream, ctypes_ref, require_cuda
+from .switch_layers import GeGLU, SwitchGLU, _contig, call_on, ctypes_ref, require_cuda
 
 
 class Router(nn.Module):
@@ -60,8 +60,8 @@ class Router(nn.Module):
         H = self.proj.weight.shape[1]
         xi = _contig(x.reshape(-1, H))
         out = torch.empty_like(xi)
-        _lib.call("vqmoe_rms_norm", xi.data_ptr(), self.norm_weight.data_ptr(), xi.shape[0], H,
-                  float(self.eps), out.data_ptr(), c_stream(x.device))
+        call_on(x.device, "vqmoe_rms_norm", xi.data_ptr(), self.norm_weight.data_ptr(), xi.shape[0], H,
+                float(self.eps), out.data_ptr())
         return out.reshape(x.shape)
 
     def forward(self, x: torch.Tensor):
@@ -75,9 +75,9 @@ class Router(nn.Module):
         scores = torch.empty((T, k), dtype=torch.float32, device=x.device)
         n = _lib.lib().vqmoe_router_workspace_size(T, E)
         ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        _lib.call("vqmoe_router_ex", xn.data_ptr(), self.proj.weight.data_ptr(), None, T, H, E, k,
-                  _lib.ROUTER_TOPK_SOFTMAX, self.per_expert_scale.data_ptr(), inds.data_ptr(),
-                  scores.data_ptr(), None, ws.data_ptr(), n, c_stream(x.device))
+        call_on(x.device, "vqmoe_router_ex", xn.data_ptr(), self.proj.weight.data_ptr(), None, T, H, E, k,
+                _lib.ROUTER_TOPK_SOFTMAX, self.per_expert_scale.data_ptr(), inds.data_ptr(),
+                scores.data_ptr(), None, ws.data_ptr(), n)
         return inds.reshape(*lead, k), scores.to(torch.bfloat16).reshape(*lead, k)
 
 
@@ -107,6 +107,6 @@ class Experts(nn.Module):
         g, u, d = sg.gate_descriptor(), sg.up_proj.descriptor(), sg.down_proj.descriptor()
         n = _lib.lib().vqmoe_moe_experts_workspace_size(ctypes_ref(g), ctypes_ref(d), T, k)
         ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        _lib.call("vqmoe_moe_experts", ctypes_ref(g), ctypes_ref(u), ctypes_ref(d), xi.data_ptr(), ii.data_ptr(),
-                  ww.data_ptr(), T, k, out.data_ptr(), ws.data_ptr(), n, c_stream(x.device))
+        call_on(x.device, "vqmoe_moe_experts", ctypes_ref(g), ctypes_ref(u), ctypes_ref(d), xi.data_ptr(),
+                ii.data_ptr(), ww.data_ptr(), T, k, out.data_ptr(), ws.data_ptr(), n)
         return out.reshape(*lead, H)

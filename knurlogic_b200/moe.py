@@ -25,7 +25,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .switch_layers import (Fp8SwitchLinear, QuantizedSwitchLinear, SwitchGLU, SwitchLinear, VQSwitchLinear, c_stream,
+from .switch_layers import (Fp8SwitchLinear, QuantizedSwitchLinear, SwitchGLU, SwitchLinear, VQSwitchLinear, call_on,
                             check_fp8_weight, require_cuda)
 
 
@@ -171,7 +171,8 @@ class SparseMoeBlock(nn.Module):
         Synchronises the current stream (`vqmoe_workspace_status`)."""
         if self._ws is None:
             return
-        _lib.call("vqmoe_workspace_status", self._ws.data_ptr(), c_stream(device or self._ws.device))
+        call_on(torch.device(device) if device is not None else self._ws.device, "vqmoe_workspace_status",
+                self._ws.data_ptr())
 
     def tp_buffers(self, tokens: int, device):
         """This rank's view of the split's symmetric buffers (`vqmoe_tp`),
@@ -213,13 +214,13 @@ class SparseMoeBlock(nn.Module):
             raise TypeError("the expert split writes a bf16 output")
         if self.sharding_group is not None and self.tp_reduce == "p2p" and out.dtype == torch.bfloat16:
             tp = self.tp_buffers(T, x2d.device)
-            _lib.call("vqmoe_sparse_moe_block_ep" if self.expert_split else "vqmoe_sparse_moe_block_tp",
-                      ctypes.byref(b), ctypes.byref(tp), x2d.data_ptr(), T, out.data_ptr(), ws.data_ptr(),
-                      ws.numel(), c_stream(x2d.device))
+            call_on(x2d.device, "vqmoe_sparse_moe_block_ep" if self.expert_split else "vqmoe_sparse_moe_block_tp",
+                    ctypes.byref(b), ctypes.byref(tp), x2d.data_ptr(), T, out.data_ptr(), ws.data_ptr(),
+                    ws.numel())
             return out
         odt = _lib.OUT_F32 if out.dtype == torch.float32 else _lib.OUT_BF16
-        _lib.call("vqmoe_sparse_moe_block", ctypes.byref(b), x2d.data_ptr(), T,
-                  out.data_ptr(), odt, ws.data_ptr(), ws.numel(), c_stream(x2d.device))
+        call_on(x2d.device, "vqmoe_sparse_moe_block", ctypes.byref(b), x2d.data_ptr(), T,
+                out.data_ptr(), odt, ws.data_ptr(), ws.numel())
         return out
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:

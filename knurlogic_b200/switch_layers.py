@@ -25,15 +25,23 @@ from torch import nn
 from . import _lib
 
 
-def _stream(t: torch.Tensor):
-    return c_stream(t.device)
-
-
 def c_stream(device) -> int:
     i = device.index if isinstance(device, torch.device) else None
     if i is None:
         return torch.cuda.current_stream(device).cuda_stream
     return torch._C._cuda_getCurrentRawStream(i)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """An entry point on `device` and its current stream (the last argument),
+    whichever device is the current one: the stream's handle alone does not
+    say (every device's default stream has the same)."""
+    i = device.index
+    if i is None or i == torch.cuda.current_device():
+        _lib.call(name, *args, c_stream(device))
+    else:
+        with torch.cuda.device(i):
+            _lib.call(name, *args, c_stream(device))
 
 
 def require_cuda(*ts: torch.Tensor) -> None:
@@ -104,9 +112,8 @@ class _SwitchBase(nn.Module):
         d = self.descriptor()
         n = _lib.lib().vqmoe_switch_linear_workspace_size(ctypes_ref(d), tokens, k, per_pair)
         ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-        _lib.call("vqmoe_switch_linear", ctypes_ref(d), xi.data_ptr(),
-                  per_pair, ii.data_ptr(), tokens, k, y.data_ptr(), ws.data_ptr(), n,
-                  _stream(x))
+        call_on(x.device, "vqmoe_switch_linear", ctypes_ref(d), xi.data_ptr(),
+                per_pair, ii.data_ptr(), tokens, k, y.data_ptr(), ws.data_ptr(), n)
         return y.reshape(*B, 1, self.output_dims)
 
 
@@ -235,8 +242,8 @@ class VQSwitchLinear(_SwitchBase):
             E, OUT, W = c.shape
             K, dim = (int(n) for n in self.codebook.shape)
             bad = torch.zeros(1, dtype=torch.int32, device=c.device)
-            _lib.call("vqmoe_count_bad_codes" if c.dtype == torch.uint8 else "vqmoe_count_bad_codes_u16",
-                      c.data_ptr(), c.numel(), K, bad.data_ptr(), _stream(c))
+            call_on(c.device, "vqmoe_count_bad_codes" if c.dtype == torch.uint8 else "vqmoe_count_bad_codes_u16",
+                    c.data_ptr(), c.numel(), K, bad.data_ptr())
             n_bad = int(bad.item())
             if n_bad:
                 raise ValueError(f"{n_bad} VQ codes are >= the codebook size {K}")
@@ -247,8 +254,8 @@ class VQSwitchLinear(_SwitchBase):
             nc, ns = _lib.vq_layout_bytes(E, OUT, IN)
             dc = torch.empty(nc, dtype=torch.uint8, device=c.device)
             ds = torch.empty(ns // 2, dtype=torch.float16, device=c.device)
-            _lib.call("vqmoe_prepare_vq", c.data_ptr(), vs.data_ptr(), E, OUT, IN,
-                      dc.data_ptr(), ds.data_ptr(), _stream(c))
+            call_on(c.device, "vqmoe_prepare_vq", c.data_ptr(), vs.data_ptr(), E, OUT, IN,
+                    dc.data_ptr(), ds.data_ptr())
             self._dev = (key, dc, ds)
         return self._dev[1], self._dev[2]
 
@@ -287,8 +294,7 @@ class VQSwitchLinear(_SwitchBase):
         out = torch.empty((count, self.output_dims, self.input_dims),
                           dtype=torch.float16, device=self.codebook.device)
         d = self.descriptor()
-        _lib.call("vqmoe_dequant", ctypes_ref(d), first, count, out.data_ptr(),
-                  _stream(out))
+        call_on(out.device, "vqmoe_dequant", ctypes_ref(d), first, count, out.data_ptr())
         return out
 
 
@@ -354,7 +360,7 @@ class QuantizedSwitchLinear(_SwitchBase):
         out = torch.empty((count, self.output_dims, self.input_dims), dtype=torch.bfloat16,
                           device=self.weight.device)
         d = self.descriptor()
-        _lib.call("vqmoe_dequant", ctypes_ref(d), first, count, out.data_ptr(), _stream(out))
+        call_on(out.device, "vqmoe_dequant", ctypes_ref(d), first, count, out.data_ptr())
         return out
 
 
@@ -508,7 +514,6 @@ class SwitchGLU(nn.Module):
         y = x.new_empty((T, k, d.out_features))
         ws_bytes = _lib.lib().vqmoe_switch_glu_workspace_size(ctypes_ref(g), ctypes_ref(d), T, k)
         ws = x.new_empty(ws_bytes, dtype=torch.uint8)
-        _lib.call("vqmoe_switch_glu", ctypes_ref(g), ctypes_ref(u), ctypes_ref(d),
-                  xi.data_ptr(), ii.data_ptr(), T, k, y.data_ptr(), ws.data_ptr(),
-                  ws_bytes, _stream(x))
+        call_on(x.device, "vqmoe_switch_glu", ctypes_ref(g), ctypes_ref(u), ctypes_ref(d),
+                xi.data_ptr(), ii.data_ptr(), T, k, y.data_ptr(), ws.data_ptr(), ws_bytes)
         return y.reshape(*lead, k, -1)

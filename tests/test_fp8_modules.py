@@ -119,8 +119,8 @@ def test_a_captured_first_call_has_a_status_word(monkeypatch, place):
     m, x = place(), make_x(3, 272, 1, DEV)
     assert list(fp8._status) == [0]
     given = []
-    call = fp8._call_on
-    monkeypatch.setattr(fp8, "_call_on", lambda dev, name, *a: (given.append(a[-1]), call(dev, name, *a)))
+    call = fp8.call_on
+    monkeypatch.setattr(fp8, "call_on", lambda dev, name, *a: (given.append(a[-1]), call(dev, name, *a)))
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         y = m(x)
