@@ -24,7 +24,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from .switch_layers import GeGLU, SwitchGLU, _contig, call_on, ctypes_ref, require_cuda
+from .switch_layers import GeGLU, SwitchGLU, _contig, call_on, check_devices, ctypes_ref, require_cuda
 
 
 class Router(nn.Module):
@@ -96,6 +96,9 @@ class Experts(nn.Module):
         if x.dtype != torch.bfloat16:
             raise TypeError(f"x must be bfloat16, got {x.dtype}")
         sg = self.switch_glu
+        check_devices(x, top_k_indices, sg.gate_proj, sg.up_proj, sg.down_proj)
+        if top_k_weights.device != x.device:
+            raise ValueError(f"top_k_weights are on {top_k_weights.device}, x on {x.device}")
         H = sg.gate_proj.input_dims
         k = top_k_indices.shape[-1]
         lead = x.shape[:-1]

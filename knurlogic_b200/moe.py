@@ -26,7 +26,7 @@ from torch import nn
 
 from . import _lib
 from .switch_layers import (Fp8SwitchLinear, QuantizedSwitchLinear, SwitchGLU, SwitchLinear, VQSwitchLinear, call_on,
-                            check_fp8_weight, require_cuda)
+                            check_devices, check_fp8_weight, require_cuda)
 
 
 def _bf16_linear(weight: torch.Tensor) -> nn.Linear:
@@ -208,6 +208,8 @@ class SparseMoeBlock(nn.Module):
         Under a split with `tp_reduce="p2p"` (bf16 `out`) the result is the
         whole split's, reduced over peer memory."""
         T = x2d.shape[0]
+        sm = self.switch_mlp._modules
+        check_devices(x2d, None, sm["gate_proj"], sm["up_proj"], sm["down_proj"])
         b = self._desc()
         ws = self.workspace(T, x2d.device)
         if self.expert_split and out.dtype != torch.bfloat16:

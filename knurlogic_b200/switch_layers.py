@@ -18,6 +18,8 @@ Every call runs on the CUDA path; there is no CPU implementation.
 """
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import torch
 from torch import nn
@@ -54,6 +56,17 @@ def require_cuda(*ts: torch.Tensor) -> None:
                 f"path); got a tensor on {t.device}")
 
 
+def check_devices(x: torch.Tensor, indices: torch.Tensor | None, *linears) -> None:
+    """A launch takes addresses: indices and expert weights of another device
+    than x's are refused."""
+    dev = x.device
+    if indices is not None and indices.device != dev:
+        raise ValueError(f"indices are on {indices.device}, x on {dev}")
+    for w in linears:
+        if w.device != dev:
+            raise ValueError(f"{type(w).__name__}'s weights are on {w.device}, x on {dev}")
+
+
 def _contig(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
@@ -68,6 +81,10 @@ class _SwitchBase(nn.Module):
     def descriptor(self) -> _lib.Linear:           # pragma: no cover
         raise NotImplementedError
 
+    @property
+    def device(self) -> torch.device:              # where the kernels' weights are
+        return self._buffers["weight"].device
+
     def _x_dtype(self):
         return torch.bfloat16
 
@@ -81,6 +98,7 @@ class _SwitchBase(nn.Module):
         form `_gather_sort` makes). `sorted_indices` is accepted for the
         reference's signature; the kernel groups pairs by expert itself."""
         require_cuda(x, indices)
+        check_devices(x, indices, self)
         if x.dtype != torch.bfloat16:
             raise TypeError(f"x must be bfloat16, got {x.dtype}")
         if x.shape[-1] != self.input_dims:
@@ -117,9 +135,7 @@ class _SwitchBase(nn.Module):
         return y.reshape(*B, 1, self.output_dims)
 
 
-def ctypes_ref(s):
-    import ctypes
-    return ctypes.byref(s)
+ctypes_ref = ctypes.byref
 
 
 class SwitchLinear(_SwitchBase):
@@ -131,6 +147,10 @@ class SwitchLinear(_SwitchBase):
             raise ValueError(f"weight must be [E, OUT, IN], got {tuple(weight.shape)}")
         self.weight = nn.Parameter(weight.to(torch.bfloat16).contiguous(),
                                    requires_grad=False)
+
+    @property
+    def device(self) -> torch.device:
+        return self.weight.device
 
     @property
     def num_experts(self):
@@ -213,6 +233,10 @@ class VQSwitchLinear(_SwitchBase):
         self.register_buffer("codebook", codebook.to(torch.float16).contiguous())
         self.register_buffer("vq_scales", vq_scales.to(torch.float16).contiguous())
         self._dev = None          # (device, data_ptr, prepared codes)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codebook.device
 
     @property
     def num_experts(self):
@@ -386,8 +410,8 @@ def fp8_descriptor(module: Fp8Buffers) -> _lib.Linear:
     or by one of another shape where the last one lay (the caller changes
     nothing in the descriptor)."""
     w, s = module._buffers["weight"], module._buffers["weight_scale_inv"]
-    key = (w.data_ptr(), s.data_ptr(), w.shape, s.shape, w.dtype, s.dtype, w.device, s.device, w.is_contiguous(),
-           s.is_contiguous())
+    key = (w.data_ptr(), s.data_ptr(), w.shape, s.shape, w.dtype, s.dtype, w.get_device(), s.get_device(),
+           w.is_contiguous(), s.is_contiguous())
     held = module.__dict__.get("_descriptor")
     if held is None or held[0] != key:
         check_fp8_weight(w, s, module.weight_dims)
@@ -504,6 +528,7 @@ class SwitchGLU(nn.Module):
         if x.dtype != torch.bfloat16:
             raise TypeError(f"x must be bfloat16, got {x.dtype}")
         m = self._modules
+        check_devices(x, indices, m["gate_proj"], m["up_proj"], m["down_proj"])
         g, u, d = self.gate_descriptor(), m["up_proj"].descriptor(), m["down_proj"].descriptor()
         H = g.in_features
         k = indices.shape[-1]

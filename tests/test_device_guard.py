@@ -66,3 +66,33 @@ def test_every_module_calls_on_its_inputs_device(monkeypatch):
                                     "vqmoe_router_ex", "vqmoe_sparse_moe_block", "vqmoe_workspace_status",
                                     "vqmoe_grouped_linear", "vqmoe_quantize_fp8", "vqmoe_add_rms_norm"]
     assert all(d == x.device for _, d in seen)
+
+
+def test_tensors_of_two_devices_are_refused(monkeypatch):
+    """(The meta device stands in for a second GPU.)"""
+    for m in (switch_layers, gemma4, moe):
+        monkeypatch.setattr(m, "call_on", lambda *a: pytest.fail("launched"))
+        monkeypatch.setattr(m, "require_cuda", lambda *ts: None)
+    E, k, H, I = 8, 2, 256, 128
+    cfgs = [synth.MoEConfig(q, E, k, H, I, 0, 3, quant=q) for q in ("vq", "affine", "fp8")]
+    cfgs.append(synth.MoEConfig("dense", E, k, H, I, 0, 3, quant="dense"))
+    x, idx = torch.zeros(3, H, dtype=torch.bfloat16), torch.zeros(3, k, dtype=torch.int32)
+    for cfg in cfgs:
+        if cfg.quant == "dense":
+            sw = [switch_layers.SwitchLinear(torch.zeros(s)) for s in ((E, I, H), (E, I, H), (E, H, I))]
+            blk = SparseMoeBlock(torch.zeros(E, H), SwitchGLU(*sw), k)
+        else:
+            blk = SparseMoeBlock.from_weights(synth.make_weights(cfg, seed=1), k)
+        glu = blk.switch_mlp
+        with pytest.raises(ValueError, match="indices are on meta"):
+            glu(x, idx.to("meta"))
+        with pytest.raises(ValueError, match="indices are on meta"):
+            glu.gate_proj(x.view(3, 1, 1, H), idx.to("meta"))
+        glu.down_proj.to("meta")
+        for call in (lambda: glu(x, idx), lambda: blk(x),
+                     lambda: glu.down_proj(torch.zeros(3, 1, 1, I, dtype=torch.bfloat16), idx)):
+            with pytest.raises(ValueError, match="weights are on meta"):
+                call()
+        e = gemma4.Experts(SwitchGLU(glu.gate_proj, glu.up_proj, glu.down_proj, activation=GeGLU()))
+        with pytest.raises(ValueError, match="weights are on meta"):
+            e(x, idx, torch.ones(3, k))
